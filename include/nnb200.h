@@ -9,7 +9,7 @@
  * There is no CPU fallback: without a CUDA device every compute entry point fails.
  *
  * Section 1 re-exports, symbol for symbol, the fifteen kernels of cuda/cuda_kernels.h so the
- * reference CudaBackend links against this library unchanged.  Sections 2-5 are new entry points in
+ * reference CudaBackend links against this library unchanged.  Sections 2-6 are new entry points in
  * the same style for what the reference CudaEngine leaves unimplemented or composes from many
  * primitive calls.
  */
@@ -445,6 +445,78 @@ int nnb200_rt_sync(void);
  * time since _start in milliseconds.  The reference times its loop on the host clock (text_train.cpp:1107). */
 int nnb200_rt_timer_start(void);
 int nnb200_rt_timer_stop(float* host_ms);
+
+/* ===================================================================================== *
+ * 6. Batched decoding over a paged key / value cache                                     *
+ * ===================================================================================== */
+
+/* Several continuations of one prompt, or of several, decoded together: beam search, several samples, a batch of requests
+ * behind one long prompt.  The reference decodes one sequence at a time from a cache of its own per layer
+ * (GPTModel::generate, compute_layer.hpp:2952-3096); none of these entry points has a counterpart there.
+ *
+ * The cache: `layers` pools of `pages` pages for keys and as many for values, layer l's at k + l * layer_stride elements, a
+ * page (kv_heads, page_size, head_dim).  Row t of a sequence is row t % page_size of page table[t / page_size], its page
+ * table being a row of page numbers in device memory.  dtype 0 = fp32, 1 = bf16; page_size a power of two from 8 to 256,
+ * head_dim a multiple of 8 up to 256; k and v 16-byte aligned, layer_stride a multiple of 8 (not read when layers is 1).
+ * Lengths, positions and page numbers are device data, which no call checks on the host: every kernel takes a page number
+ * outside [0, pages) for a page that is not there, and nothing outside the pools and the arguments is read or written.
+ * The struct itself is host memory and read before a call returns. */
+typedef struct nnb200_paged_kv {
+    void* k;
+    void* v;
+    int64_t layer_stride;
+    int32_t layers, pages, page_size, kv_heads, head_dim, dtype;
+    int32_t reserved[2];
+} nnb200_paged_kv;
+
+/* Appends `tokens` new rows to layer `layer`: token i's keys and values (k + i * ldkv, kv_heads * head_dim values, the same
+ * for v; type src_dtype) go to row row_of[i] of sequence seq_of[i] (NULL: sequence i), in the pages of row seq_of[i] of
+ * page_table (seqs, table_stride).  rope (NULL = none): the table of nnb200_rope_table for rope_len positions; keys and
+ * queries are rotated to position rope_pos[i] (NULL: row_of[i]) on the way, as nnb200_rope_apply does.  Queries (q, rows of
+ * `heads` * head_dim values of type src_dtype; NULL = none) go to q_out in the cache's type; q_out = q rotates in place
+ * (same type and stride).  Products in fp32, one rounding to the cache's type.  A token whose sequence, row, page or position
+ * does not exist is left out: its q_out row stays as it was.  Two tokens for one row leave a mixture of the two there. */
+int nnb200_paged_append(const nnb200_paged_kv* kv, int layer, const void* q, long long ldq, void* q_out, long long ldqo, const void* k,
+                        const void* v, long long ldkv, int src_dtype, int tokens, int heads, const int32_t* seq_of, const int32_t* row_of,
+                        const int32_t* page_table, int seqs, int table_stride, const float* rope, int rope_len, const int32_t* rope_pos,
+                        void* stream);
+/* One query per sequence over a shared prefix and the sequence's own rows.  Sequence i (of groups * group_size) belongs to
+ * group g = i / group_size and sees rows [0, prefix_len[g]) of the pages in row g of prefix_table (groups, prefix_stride),
+ * then rows [0, seq_len[i]) of those in row i of page_table (.., table_stride); seq_len[i] < 0: nothing at all (a padded
+ * sequence).  The prefix is read once for the group.  heads is a multiple of the cache's kv_heads (query head h reads head
+ * h / (heads / kv_heads)); scores are scaled by 1 / sqrt(head_dim); alibi: minus slope_h times the distance to the last row
+ * seen, slope_h = 2^(-8 h / heads) as in nnb200_attention_forward.  q, out: rows of heads * head_dim values of the cache's type
+ * with strides ldq, ldo; lse (NULL, or groups * group_size * heads): log of the sum of exponentials.  A query for which no row
+ * has weight gives 0 and -inf.  Lengths beyond what the page tables hold count as what they hold; a stride of 0 is no prefix,
+ * or no rows.  Accumulation and softmax in fp32; bf16: the weights are rounded to bf16 for their product with the values.
+ * scratch (16-byte aligned): nnb200_paged_attention_scratch_bytes, nothing in it needs to be set or kept; two calls that may
+ * overlap need one each. */
+size_t nnb200_paged_attention_scratch_bytes(const nnb200_paged_kv* kv, int groups, int group_size, int heads, int prefix_stride,
+                                            int table_stride);
+int nnb200_paged_attention(const nnb200_paged_kv* kv, int layer, const void* q, long long ldq, void* out, long long ldo, float* lse,
+                           const int32_t* prefix_table, int prefix_stride, const int32_t* prefix_len, const int32_t* page_table,
+                           int table_stride, const int32_t* seq_len, int groups, int group_size, int heads, int alibi, void* scratch,
+                           size_t scratch_bytes, void* stream);
+/* Beam search's selection.  logits: groups * beams rows of vocab values (stride ld; dtype 0 fp32, 1 bf16); scores: the beams'
+ * summed log-probabilities so far.  For each group the n (1..128) best continuations (beam b, token v) by
+ * scores[b] + logits[b][v] - log(sum(exp(logits[b]))), best first, equal ones in order of (b, v): parent (beam within the
+ * group), token, scores_out and ended_out (may be NULL), each (groups, n).  A beam with ended[b] != 0 (NULL: none) has one continuation: the
+ * token eos at its own score.  ended_out: the parent had ended, or the token is eos (-1: no such token).  -inf and NaN values
+ * are no continuations, nor is anything of a row that holds NaN or +inf; places that nothing is left for get parent -1,
+ * token -1, score -inf.  Up to 64 beams.  Values are compared in 64 bits; the normaliser is summed in 64 bits from
+ * exponentials in 32. */
+size_t nnb200_beam_select_scratch_bytes(int groups, int beams, int vocab, int n);
+int nnb200_beam_select(const void* logits, long long ld, int dtype, int groups, int beams, int vocab, const float* scores,
+                       const int32_t* ended, int eos, int n, int32_t* parent, int32_t* token, float* scores_out, int32_t* ended_out,
+                       void* scratch, size_t scratch_bytes, void* stream);
+/* Reorders the cached states of groups * beams sequences to their parents (the group's beam parent[i]; out of range: i's own):
+ * len_out[i] = len[p]; page_table_out[i] = page_table[p] for the whole pages, which the sequences then share and none writes
+ * again; the page that is partly filled is copied in every layer into page spare[i], which takes its place in
+ * page_table_out[i]; the entries behind it stay i's own.  spare_out[i]: the page i gives up for it, to be the next call's spare
+ * (spare[i] itself where no page was partly filled).  The new tables must not be the old ones.  The beams of a group have one
+ * length, and every sequence pages of its own for the rows to come: with these, nothing that two sequences share is written. */
+int nnb200_beam_reorder(const nnb200_paged_kv* kv, int groups, int beams, const int32_t* parent, const int32_t* len, const int32_t* page_table,
+                        const int32_t* spare, int32_t* len_out, int32_t* page_table_out, int32_t* spare_out, int table_stride, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,12 @@ class GptConfigC(C.Structure):
                                           "norm", "pos", "precision")] + [("reserved", C.c_int32 * 5)]
 
 
+class PagedKv(C.Structure):
+    """struct nnb200_paged_kv (include/nnb200.h): the paged key / value cache of batched decoding.  k, v: device addresses."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("layer_stride", C.c_int64)] + [
+        (n, C.c_int32) for n in ("layers", "pages", "page_size", "kv_heads", "head_dim", "dtype")] + [("reserved", C.c_int32 * 2)]
+
+
 def _load():
     if not os.path.isfile(LIB_PATH):
         raise ImportError(
@@ -31,7 +37,7 @@ def _load():
 lib = _load()
 
 _p, _i, _u, _f, _ll, _sz = C.c_void_p, C.c_int, C.c_uint, C.c_float, C.c_longlong, C.c_size_t
-_cfgp = C.POINTER(GptConfigC)
+_cfgp, _kvp = C.POINTER(GptConfigC), C.POINTER(PagedKv)
 
 # name -> argument types; every function returns int unless listed in _RET
 SIGNATURES = {
@@ -109,6 +115,13 @@ SIGNATURES = {
     "nnb200_gpt_forward": [_cfgp, _p, _p, _p, _p, _p, _p],
     "nnb200_gpt_loss": [_cfgp, _p, _p, _p, _f, _p],
     "nnb200_gpt_backward": [_cfgp, _p, _p, _p, _p, _p, _p, _p, _p],
+    # batched decoding over a paged cache
+    "nnb200_paged_append": [_kvp, _i, _p, _ll, _p, _ll, _p, _p, _ll, _i, _i, _i, _p, _p, _p, _i, _i, _p, _i, _p, _p],
+    "nnb200_paged_attention_scratch_bytes": [_kvp, _i, _i, _i, _i, _i],
+    "nnb200_paged_attention": [_kvp, _i, _p, _ll, _p, _ll, _p, _p, _i, _p, _p, _i, _p, _i, _i, _i, _i, _p, _sz, _p],
+    "nnb200_beam_select_scratch_bytes": [_i, _i, _i, _i],
+    "nnb200_beam_select": [_p, _ll, _i, _i, _i, _i, _p, _p, _i, _i, _p, _p, _p, _p, _p, _sz, _p],
+    "nnb200_beam_reorder": [_kvp, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i, _p],
     # engine primitives in the reference's layouts
     "nnb200_batched_matmul": [_p, _p, _p, _sz, _sz, _sz, _sz, _u, _i, _i, _f, _p],
     "nnb200_bmm_reduce": [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p],
@@ -142,6 +155,7 @@ _RET = {
     "nnb200_muon_scratch_bytes": _sz, "nnb200_gpt_arena_elems": _ll, "nnb200_gpt_matrix_region_begin": _ll,
     "nnb200_gpt_layer_matrix_begin": _ll, "nnb200_gpt_workspace_bytes": _ll, "nnb200_gpt_workspace_offset": _ll,
     "nnb200_gpt_decode_workspace_bytes": _ll,
+    "nnb200_paged_attention_scratch_bytes": _sz, "nnb200_beam_select_scratch_bytes": _sz,
     "nnb200_eval_expr_scratch_floats": _sz, "nnb200_rt_stream": C.c_void_p,
 }
 # functions whose int return value is a count, not a status
