@@ -3,7 +3,16 @@
 //   s_t = q . k_t / sqrt(dk) - slope_h (T - 1 - t),  out = sum_t softmax(s)_t v_t,  lse = log sum_t exp(s_t)
 // with t over the T = prefix_len + seq_len rows the query sees; a query for which no row has weight (it sees none, or all
 // its scores are -inf) gives 0 and -inf.
+//
+// A group's queries that read one head of the cache are the rows of one tile, so the prefix is read once for all of them; own
+// rows are read by the query heads that share them.  Both are the same task, "rows of queries against a run of cached rows":
+// the runs are split over blocks until the machine is full, each block leaves its unnormalised sums with their maximum and
+// sum of exponentials in scratch, and a second kernel, already resident when the last block ends, joins them in fixed order.
 #include "paged.cuh"
+#include "tc_ptx.cuh"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace nnb {
 
@@ -14,70 +23,528 @@ struct PagedAttnArgs {
     long long ldq, ldo;
     const int *prefix_table, *prefix_len, *table, *len;
     int prefix_stride, table_stride, groups, size, heads, alibi;
+    int m;                          // query heads per cached head
+    int row_tiles, own_tiles;       // tiles of a group's rows, of a sequence's
+    int pre_splits, own_splits;     // blocks that share a prefix, a sequence's own rows
+    long long pre_blocks;           // blocks [0, pre_blocks) take prefixes, the others own rows
+    int pairs;                      // queries may be read two columns at a time
+    float c;                        // log2(e) / sqrt(head_dim): exponentials are powers of two
+    float* part;                    // (query row, slot): head_dim sums
+    float2* stat;                   // (query row, slot): maximum (in powers of two) and sum; sum 0: nothing there
+    __host__ __device__ int slots() const { return pre_splits + own_splits; }
 };
 
-// A block per (sequence, query head): warps take rows in turn, a lane every 32nd column, partial softmax states joined at the end.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attn_kernel(PagedPool<T> pool, PagedAttnArgs a, float scale)
+__device__ __forceinline__ float exp2_fast(float x)
 {
-    constexpr int C = 8, WARPS = 4;
-    const int seq = blockIdx.x, h = blockIdx.y, hk = h / (a.heads / pool.kv_heads), g = seq / a.size;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dk = pool.dk, ps = 1 << pool.page_shift;
-    const int own = a.table_stride ? a.len[seq] : min(a.len[seq], 0);
-    const long long own_cap = static_cast<long long>(a.table_stride) << pool.page_shift, pre_cap = static_cast<long long>(a.prefix_stride) << pool.page_shift;
-    const int n_own = static_cast<int>(min(static_cast<long long>(max(own, 0)), own_cap));
-    const int n_pre = own < 0 || !a.prefix_stride ? 0 : static_cast<int>(min(static_cast<long long>(max(a.prefix_len[g], 0)), pre_cap));
-    const T* qp = static_cast<const T*>(a.q) + seq * a.ldq + static_cast<long long>(h) * dk;
-    float q[C], o[C], m = -INFINITY, l = 0.f;
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float alibi_slope2(int h, int heads) { return exp2f(-8.0f * static_cast<float>(h) / static_cast<float>(heads)) * 1.4426950408889634f; }
+
+// What a block works on: `rows` query rows (row r is query head head0 + r % m of sequence seq0 + r / m) against rows
+// [begin, end) of one page table.  Row t stands at position place + t of what sequence `seq` sees in all.
+struct AttnTask {
+    const int* table;
+    int hk, first, rows, begin, end, place, slot, group;
+};
+// lengths are device data: clamped to [0, what the table holds]; negative own length: nothing is seen
+__device__ __forceinline__ int held(int len, int stride, int shift)
+{
+    return static_cast<int>(min(static_cast<long long>(max(len, 0)), static_cast<long long>(stride) << shift));
+}
+// the share of split s: whole tiles of 64 rows, so that few rows go to few splits
+__device__ __forceinline__ void share_of(int len, int splits, int s, int& begin, int& end)
+{
+    const int per = ((len + splits - 1) / splits + 63) & ~63;
+    begin = static_cast<int>(min(static_cast<long long>(s) * per, static_cast<long long>(len)));
+    end = min(len - begin, per) + begin;
+}
+template <int RT, typename T>
+__device__ __forceinline__ AttnTask task_of(const PagedPool<T>& pool, const PagedAttnArgs& a, long long b)
+{
+    AttnTask k;
+    if (b < a.pre_blocks) {                                     // neighbours share their cached rows: row tiles, then splits
+        const int rt = static_cast<int>(b % a.row_tiles); b /= a.row_tiles;
+        const int s = static_cast<int>(b % a.pre_splits); b /= a.pre_splits;
+        k.hk = static_cast<int>(b % pool.kv_heads);
+        const int g = static_cast<int>(b / pool.kv_heads);
+        k.group = g;
+        k.first = rt * RT;
+        k.rows = min(a.size * a.m - k.first, RT);
+        k.table = a.prefix_table + static_cast<long long>(g) * a.prefix_stride;
+        k.place = 0;
+        k.slot = s;
+        share_of(held(a.prefix_len[g], a.prefix_stride, pool.page_shift), a.pre_splits, s, k.begin, k.end);
+        return k;
+    }
+    b -= a.pre_blocks;
+    const int rt = static_cast<int>(b % a.own_tiles); b /= a.own_tiles;
+    const int s = static_cast<int>(b % a.own_splits); b /= a.own_splits;
+    k.hk = static_cast<int>(b % pool.kv_heads);
+    const int seq = static_cast<int>(b / pool.kv_heads);
+    k.group = seq / a.size;
+    k.first = (seq - k.group * a.size) * a.m + rt * 16;
+    k.rows = min(a.m - rt * 16, 16);
+    k.table = a.table + static_cast<long long>(seq) * a.table_stride;
+    k.place = a.prefix_stride ? held(a.prefix_len[k.group], a.prefix_stride, pool.page_shift) : 0;
+    k.slot = a.pre_splits + s;
+    share_of(held(a.len[seq], a.table_stride, pool.page_shift), a.own_splits, s, k.begin, k.end);
+    return k;
+}
+__device__ __forceinline__ int seq_of_row(const PagedAttnArgs& a, const AttnTask& k, int r) { return k.group * a.size + (k.first + r) / a.m; }
+__device__ __forceinline__ int head_of_row(const PagedAttnArgs& a, const AttnTask& k, int r) { return k.hk * a.m + (k.first + r) % a.m; }
+// distance from row `place + t` to the last one the query sees is far_of - t
+__device__ __forceinline__ int far_of(const PagedAttnArgs& a, int shift, const AttnTask& k, int r)
+{
+    const int seq = seq_of_row(a, k, r);
+    const int pre = a.prefix_stride ? held(a.prefix_len[k.group], a.prefix_stride, shift) : 0;
+    return pre + (a.table_stride ? held(a.len[seq], a.table_stride, shift) : 0) - 1 - k.place;
+}
+
+// ---------------------------------------------------------------- bf16: mma.sync tiles
+// 64 cached rows a step, a ring of STAGES steps filled by 16-byte asynchronous copies; WM warps take 16 query rows each, the
+// 4 / WM warps of a set of rows take turns at the step's cached rows and are joined at the end.  Cached rows that do not
+// exist are zero in shared memory (what lies there may be anything, and zero times it must be zero) and -inf as scores.
+template <int DP> struct AttnTile {
+    static constexpr int KT = 64, CPR = DP / 8;                // cached rows a step, 16-byte chunks a row
+    static constexpr int STAGES = DP <= 64 ? 4 : (DP == 128 ? 3 : 2);
+    static constexpr int BYTES = KT * DP * 2;
+    static constexpr int SMEM = STAGES * 2 * BYTES + STAGES * (KT + 16) + 64;
+    // chunk c of row r: eight rows of one chunk column fall into eight different 16-byte banks
+    static __device__ __forceinline__ uint32_t at(int r, int c)
+    {
+        return static_cast<uint32_t>(r * (DP * 2) + ((CPR >= 8 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
+    }
+};
+
+template <int DP> struct AttnLoader {
+    using Tile = AttnTile<DP>;
+    const PagedPool<bf16>& pool;
+    const AttnTask& k;
+    uint32_t base;                  // shared memory: K, V of each stage
+    uint8_t* alive;                 // per stage: KT flags, then one per warp for "some row of the step is not there"
+    __device__ __forceinline__ void load(int step, int stage) const
+    {
+        const int t0 = k.begin + step * Tile::KT, tid = threadIdx.x;
+        bool gap = false;
 #pragma unroll
-    for (int i = 0; i < C; ++i) { const int c = lane + 32 * i; q[i] = c < dk ? to_f32(qp[c]) : 0.f; o[i] = 0.f; }
-    const float slope = a.alibi ? exp2f(-8.0f * static_cast<float>(h) / static_cast<float>(a.heads)) : 0.f;
-    const int total = n_pre + n_own;
-    for (int t = warp; t < total; t += WARPS) {
-        const int r = t < n_pre ? t : t - n_pre;
-        const int* table = t < n_pre ? a.prefix_table + static_cast<long long>(g) * a.prefix_stride : a.table + static_cast<long long>(seq) * a.table_stride;
-        const int page = table[r >> pool.page_shift];
-        if (page < 0 || page >= pool.pages) continue;
-        const long long at = pool.at(page, hk, r & (ps - 1));
-        float s = 0.f, v[C];
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = lane + 32 * i;
-            if (c < dk) s = fmaf(q[i], to_f32(pool.k[at + c]), s);
-            v[i] = c < dk ? to_f32(pool.v[at + c]) : 0.f;
+        for (int i = 0; i < Tile::KT * Tile::CPR / 128; ++i) {
+            const int idx = tid + i * 128, r = idx / Tile::CPR, c = idx % Tile::CPR, t = t0 + r;
+            int page = -1;
+            if (t < k.end) page = __ldg(k.table + (t >> pool.page_shift));
+            const bool there = page >= 0 && page < pool.pages;
+            const long long off = there && c * 8 < pool.dk ? pool.at(page, k.hk, t & ((1 << pool.page_shift) - 1)) + c * 8 : 0;
+            const int bytes = there && c * 8 < pool.dk ? 16 : 0;
+            const uint32_t dst = base + stage * 2 * Tile::BYTES + Tile::at(r, c);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pool.k + off), "r"(bytes) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Tile::BYTES), "l"(pool.v + off), "r"(bytes) : "memory");
+            gap |= !there;
+            if (c == 0) alive[stage * (Tile::KT + 16) + r] = there;
         }
-        s = warp_sum(s) * scale - slope * static_cast<float>(total - 1 - t);
-        const float nm = fmaxf(m, s), ref = nm == -INFINITY ? 0.f : nm, back = expf(m - ref), e = expf(s - ref);
-        m = nm;
-        l = l * back + e;
-#pragma unroll
-        for (int i = 0; i < C; ++i) o[i] = fmaf(e, v[i], o[i] * back);
+        const bool any = __any_sync(0xffffffffu, gap);
+        if ((tid & 31) == 0) alive[stage * (Tile::KT + 16) + Tile::KT + (tid >> 5)] = any;
     }
-    __shared__ float sm[WARPS], sl[WARPS], so[WARPS][256];
-    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+};
+
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t p)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t p)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Leaves a row's state: in scratch for the join, or finished where a row has one slot only.
+__device__ __forceinline__ bool sees(const PagedAttnArgs& a, int seq) { return a.len[seq] >= 0; }
+template <typename T>
+__device__ __forceinline__ void leave(const PagedAttnArgs& a, const AttnTask& k, int dk, int r, int c, float4 o, float m, float l)
+{
+    const int seq = seq_of_row(a, k, r), h = head_of_row(a, k, r);
+    const long long row = static_cast<long long>(seq) * a.heads + h;
+    if (a.slots() == 1) {
+        const bool none = l == 0.f || !sees(a, seq);
+        T* to = static_cast<T*>(a.out) + seq * a.ldo + static_cast<long long>(h) * dk + c;
+        const float inv = none ? 0.f : 1.0f / l;
+        to[0] = from_f32<T>(none ? 0.f : o.x * inv); to[1] = from_f32<T>(none ? 0.f : o.y * inv);
+        to[2] = from_f32<T>(none ? 0.f : o.z * inv); to[3] = from_f32<T>(none ? 0.f : o.w * inv);
+        if (c == 0 && a.lse) a.lse[row] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        return;
+    }
+    const long long at = row * a.slots() + k.slot;
+    *reinterpret_cast<float4*>(a.part + at * dk + c) = o;
+    if (c == 0) a.stat[at] = make_float2(m, l);
+}
+template <typename T>
+__device__ __forceinline__ void leave_nothing(const PagedAttnArgs& a, const AttnTask& k, int dk)
+{
+    for (int r = threadIdx.x; r < k.rows; r += blockDim.x) {
+        const int seq = seq_of_row(a, k, r), h = head_of_row(a, k, r);
+        if (a.slots() > 1) a.stat[(static_cast<long long>(seq) * a.heads + h) * a.slots() + k.slot] = make_float2(-INFINITY, 0.f);
+        else for (int c = 0; c < dk; c += 4) leave<T>(a, k, dk, r, c, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+    }
+}
+
+template <int DP, int WM>
+__device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const PagedAttnArgs& a, const AttnTask& k, uint8_t* smem)
+{
+    using Tile = AttnTile<DP>;
+    constexpr int WK = 4 / WM, KW = Tile::KT / WK, NT = KW / 8, ND = DP / 8, KS = DP / 16, ST = Tile::STAGES;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp / WK, wk = warp % WK, dk = pool.dk;
+    const int steps = (k.end - k.begin + Tile::KT - 1) / Tile::KT;
+    uint8_t* alive = smem + ST * 2 * Tile::BYTES;
+    const AttnLoader<DP> loader{pool, k, smem_u32(smem), alive};
 #pragma unroll
-    for (int i = 0; i < C; ++i) so[warp][lane + 32 * i] = o[i];
+    for (int i = 0; i < ST - 1; ++i) { if (i < steps) loader.load(i, i); cp_commit(); }
+
+    const int r0 = wm * 16 + (lane >> 2);                       // this thread's rows: r0 and r0 + 8
+    uint32_t qf[KS][4];
+    float slope[2] = {0.f, 0.f}, far[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = r0 + 8 * i;
+        const bool live = r < k.rows;
+        const bf16* q = static_cast<const bf16*>(a.q);
+        if (live) {
+            const int h = head_of_row(a, k, r);
+            q += seq_of_row(a, k, r) * a.ldq + static_cast<long long>(h) * dk;
+            if (a.alibi) { slope[i] = alibi_slope2(h, a.heads); far[i] = static_cast<float>(far_of(a, pool.page_shift, k, r)); }
+        }
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c = kk * 16 + j * 8 + (lane & 3) * 2;
+                uint32_t v = 0;
+                if (live && c < dk) {
+                    if (a.pairs) v = *reinterpret_cast<const uint32_t*>(q + c);
+                    else v = static_cast<uint32_t>(__bfloat16_as_ushort(q[c])) | static_cast<uint32_t>(__bfloat16_as_ushort(q[c + 1])) << 16;
+                }
+                qf[kk][j * 2 + i] = v;
+            }
+    }
+
+    float o[ND][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][j] = 0.f;
+
+    for (int step = 0; step < steps; ++step) {
+        cp_wait<ST - 2>();
+        __syncthreads();
+        const int stage = step % ST;
+        if (step + ST - 1 < steps) loader.load(step + ST - 1, (step + ST - 1) % ST);
+        cp_commit();
+        const uint32_t kb = smem_u32(smem) + stage * 2 * Tile::BYTES, vb = kb + Tile::BYTES;
+        const int key0 = wk * KW;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t b[4];
+                ldsm4(b, kb + Tile::at(key0 + n * 8 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+                mma_bf16(s[n], qf[kk], b[0], b[1]);
+                mma_bf16(s[n + 1], qf[kk], b[2], b[3]);
+            }
+        const int t0 = k.begin + step * Tile::KT + key0 + (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[n][j] *= a.c;
+                if (a.alibi) s[n][j] -= slope[j >> 1] * (far[j >> 1] - static_cast<float>(t0 + n * 8 + (j & 1)));
+            }
+        const uint8_t* al = alive + stage * (Tile::KT + 16);
+        if (*reinterpret_cast<const uint32_t*>(al + Tile::KT)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (!al[key0 + n * 8 + (lane & 3) * 2 + j]) { s[n][j] = -INFINITY; s[n][j + 2] = -INFINITY; }
+        }
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
+            top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        }
+        float ref[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ref[i] = top[i] == -INFINITY ? 0.f : top[i];
+        if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float back = exp2_fast(m[i] - ref[i]);
+                l[i] *= back;
+#pragma unroll
+                for (int n = 0; n < ND; ++n) { o[n][2 * i] *= back; o[n][2 * i + 1] *= back; }
+                m[i] = top[i];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { s[n][j] = exp2_fast(s[n][j] - ref[j >> 1]); l[j >> 1] += s[n][j]; }
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            // the weights are rounded to bf16 for the tensor cores (their sum is not): 2^-9 of a weight, what rounding V costs too
+            const uint32_t p[4] = {pack_bf16x2(s[n][0], s[n][1]), pack_bf16x2(s[n][2], s[n][3]), pack_bf16x2(s[n + 1][0], s[n + 1][1]), pack_bf16x2(s[n + 1][2], s[n + 1][3])};
+#pragma unroll
+            for (int d = 0; d < ND; d += 2) {
+                uint32_t b[4];
+                ldsm4_t(b, vb + Tile::at(key0 + n * 8 + (lane & 7) + (((lane >> 3) & 1) << 3), d + (lane >> 4)));
+                mma_bf16(o[d], p, b[0], b[1]);
+                mma_bf16(o[d + 1], p, b[2], b[3]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    // join the warps of a set of rows through shared memory, write rows with whole vectors
+    cp_wait<0>();
     __syncthreads();
-    float gm = -INFINITY, gl = 0.f;
-    for (int w = 0; w < WARPS; ++w) gm = fmaxf(gm, sm[w]);
-    const float ref = gm == -INFINITY ? 0.f : gm;
-    for (int w = 0; w < WARPS; ++w) gl += sl[w] * expf(sm[w] - ref);
-    for (int c = threadIdx.x; c < dk; c += blockDim.x) {
-        float x = 0.f;
-        for (int w = 0; w < WARPS; ++w) x = fmaf(so[w][c], expf(sm[w] - ref), x);
-        static_cast<T*>(a.out)[seq * a.ldo + static_cast<long long>(h) * dk + c] = from_f32<T>(gl == 0.f ? 0.f : x / gl);
+    constexpr int LD = DP + 8;
+    float* so = reinterpret_cast<float*>(smem);                 // (warp, 16 rows, LD)
+    float2* sml = reinterpret_cast<float2*>(so + 4 * 16 * LD);
+    static_assert(4 * 16 * LD * 4 + 4 * 16 * 8 <= ST * 2 * Tile::BYTES, "the join fits the ring");
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<float2*>(so + (warp * 16 + (lane >> 2) + 8 * i) * LD + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    if ((lane & 3) == 0) {
+        sml[warp * 16 + (lane >> 2)] = make_float2(m[0], l[0]);
+        sml[warp * 16 + (lane >> 2) + 8] = make_float2(m[1], l[1]);
     }
-    if (a.lse && threadIdx.x == 0) a.lse[static_cast<long long>(seq) * a.heads + h] = ref + logf(gl);
+    __syncthreads();
+    const int vecs = dk / 4;
+    for (int idx = threadIdx.x; idx < k.rows * vecs; idx += 128) {
+        const int r = idx / vecs, c = (idx - r * vecs) * 4, w0 = (r >> 4) * WK, rr = r & 15;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, sml[(w0 + w) * 16 + rr].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+            const float2 st = sml[(w0 + w) * 16 + rr];
+            const float e = exp2_fast(st.x - ref);
+            const float4 y = *reinterpret_cast<const float4*>(so + ((w0 + w) * 16 + rr) * LD + c);
+            sum = fmaf(st.y, e, sum);
+            x.x = fmaf(y.x, e, x.x); x.y = fmaf(y.y, e, x.y); x.z = fmaf(y.z, e, x.z); x.w = fmaf(y.w, e, x.w);
+        }
+        leave<bf16>(a, k, dk, r, c, x, top, sum);
+    }
+}
+
+template <int DP, int WM>
+__global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const AttnTask k = task_of<WM * 16>(pool, a, blockIdx.x);
+    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk); return; }
+    if (blockIdx.x < a.pre_blocks) attend_bf16<DP, WM>(pool, a, k, smem);
+    else attend_bf16<DP, 1>(pool, a, k, smem);
+}
+
+// ---------------------------------------------------------------- fp32: a block per task, a warp per cached row in turn
+template <int R>
+__global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> pool, const __grid_constant__ PagedAttnArgs a)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int C = 8, WARPS = 4;
+    const AttnTask k = task_of<R>(pool, a, blockIdx.x);
+    if (k.begin >= k.end) { leave_nothing<float>(a, k, pool.dk); return; }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dk = pool.dk, ps = 1 << pool.page_shift;
+    __shared__ float sm[WARPS], sl[WARPS], so[WARPS][256];
+    for (int r = 0; r < k.rows; ++r) {
+        const int seq = seq_of_row(a, k, r), h = head_of_row(a, k, r);
+        const float* qp = static_cast<const float*>(a.q) + seq * a.ldq + static_cast<long long>(h) * dk;
+        float q[C], o[C], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) { const int c = lane + 32 * i; q[i] = c < dk ? qp[c] : 0.f; o[i] = 0.f; }
+        const float slope = a.alibi ? alibi_slope2(h, a.heads) : 0.f;
+        const int far = far_of(a, pool.page_shift, k, r);
+        for (int t = k.begin + warp; t < k.end; t += WARPS) {
+            const int page = k.table[t >> pool.page_shift];
+            if (page < 0 || page >= pool.pages) continue;
+            const long long at = pool.at(page, k.hk, t & (ps - 1));
+            float s = 0.f, v[C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int c = lane + 32 * i;
+                if (c < dk) s = fmaf(q[i], pool.k[at + c], s);
+                v[i] = c < dk ? pool.v[at + c] : 0.f;
+            }
+            s = warp_sum(s) * a.c - slope * static_cast<float>(far - t);
+            const float nm = fmaxf(m, s), ref = nm == -INFINITY ? 0.f : nm, back = exp2f(m - ref), e = exp2f(s - ref);
+            m = nm;
+            l = l * back + e;
+#pragma unroll
+            for (int i = 0; i < C; ++i) o[i] = fmaf(e, v[i], o[i] * back);
+        }
+        __syncthreads();
+        if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+#pragma unroll
+        for (int i = 0; i < C; ++i) so[warp][lane + 32 * i] = o[i];
+        __syncthreads();
+        for (int c = threadIdx.x * 4; c < dk; c += 512) {
+            float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), sum = 0.f;
+            const float ref = top == -INFINITY ? 0.f : top;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = 0; w < WARPS; ++w) {
+                const float e = exp2f(sm[w] - ref);
+                sum = fmaf(sl[w], e, sum);
+                x.x = fmaf(so[w][c], e, x.x); x.y = fmaf(so[w][c + 1], e, x.y); x.z = fmaf(so[w][c + 2], e, x.z); x.w = fmaf(so[w][c + 3], e, x.w);
+            }
+            leave<float>(a, k, dk, r, c, x, top, sum);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- the join
+// A block per query row: groups of dk / 4 threads take the slots in turn.
+template <typename T>
+__global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int dk)
+{
+    __shared__ float sx[128 * 4], sl[128], red[32];
+    const long long row = blockIdx.x;
+    const int seq = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<long long>(seq) * a.heads), slots = a.slots();
+    const bool live = sees(a, seq);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const float2* st = a.stat + row * slots;
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < slots; i += 128) m = fmaxf(m, st[i].x);
+    m = block_max(m, red);
+    const float ref = m == -INFINITY ? 0.f : m;
+    const int vecs = dk / 4, sets = 128 / vecs, set = threadIdx.x / vecs, c = (threadIdx.x - set * vecs) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (set < sets)
+        for (int i = set; i < slots; i += sets) {
+            const float2 s = st[i];
+            if (s.y == 0.f) continue;                           // nothing was left there, not even sums
+            const float e = exp2f(s.x - ref);
+            const float4 y = *reinterpret_cast<const float4*>(a.part + (row * slots + i) * dk + c);
+            l = fmaf(s.y, e, l);
+            x.x = fmaf(y.x, e, x.x); x.y = fmaf(y.y, e, x.y); x.z = fmaf(y.z, e, x.z); x.w = fmaf(y.w, e, x.w);
+        }
+    *reinterpret_cast<float4*>(sx + threadIdx.x * 4) = x;
+    sl[threadIdx.x] = l;
+    __syncthreads();
+    if (set == 0) {
+        for (int i = 1; i < sets; ++i) {
+            const int o = (i * vecs + threadIdx.x);
+            l += sl[o];
+            x.x += sx[o * 4]; x.y += sx[o * 4 + 1]; x.z += sx[o * 4 + 2]; x.w += sx[o * 4 + 3];
+        }
+        const bool none = l == 0.f || !live;
+        const float inv = none ? 0.f : 1.0f / l;
+        T* to = static_cast<T*>(a.out) + seq * a.ldo + static_cast<long long>(h) * dk + c;
+        to[0] = from_f32<T>(none ? 0.f : x.x * inv); to[1] = from_f32<T>(none ? 0.f : x.y * inv);
+        to[2] = from_f32<T>(none ? 0.f : x.z * inv); to[3] = from_f32<T>(none ? 0.f : x.w * inv);
+        if (a.lse && threadIdx.x == 0) a.lse[row] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+}
+
+// ---------------------------------------------------------------- how the work is cut
+struct AttnPlan { int rt, row_tiles, own_tiles, pre_splits, own_splits; };
+static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int heads, int prefix_stride, int table_stride)
+{
+    AttnPlan p;
+    const int m = heads / kv.kv_heads;
+    const long long rows = static_cast<long long>(size) * m;
+    p.rt = rows <= 16 || kv.dtype == 0 ? 16 : (rows <= 32 ? 32 : 64);
+    p.row_tiles = static_cast<int>(ceil_div(rows, p.rt));
+    p.own_tiles = (m + 15) / 16;
+    const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
+    const long long pre_units = static_cast<long long>(groups) * kv.kv_heads * p.row_tiles, own_units = static_cast<long long>(groups) * size * kv.kv_heads * p.own_tiles;
+    // cached rows for a block when the tables are full: enough blocks for the machine a few times over, at least two steps each
+    const long long blocks = 148LL * 8;
+    long long chunk = ceil_div(pre_units * pre + own_units * own, blocks);
+    chunk = std::min<long long>(std::max<long long>(ceil_div(chunk, 64) * 64, 128), 1 << 20);
+    p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
+    p.own_splits = static_cast<int>(ceil_div(own, chunk));
+    return p;
 }
 
 template <typename T>
-static int attention_t(const nnb200_paged_kv& kv, int layer, const PagedAttnArgs& a, cudaStream_t s)
+static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, const AttnPlan& p, void* scratch, cudaStream_t s)
 {
-    const dim3 grid(static_cast<unsigned>(a.groups * a.size), static_cast<unsigned>(a.heads));
-    paged_attn_kernel<T><<<grid, 128, 0, s>>>(paged_pool<T>(kv, layer), a, 1.0f / sqrtf(static_cast<float>(kv.head_dim)));
+    const PagedPool<T> pool = paged_pool<T>(kv, layer);
+    const long long rows = static_cast<long long>(a.groups) * a.size * a.heads;
+    a.m = a.heads / kv.kv_heads;
+    a.row_tiles = p.row_tiles; a.own_tiles = p.own_tiles; a.pre_splits = p.pre_splits; a.own_splits = p.own_splits;
+    a.pre_blocks = static_cast<long long>(a.groups) * kv.kv_heads * p.row_tiles * p.pre_splits;
+    a.c = 1.4426950408889634f / sqrtf(static_cast<float>(kv.head_dim));
+    a.pairs = ((reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.ldq % 2 == 0) ? 1 : 0;
+    a.stat = static_cast<float2*>(scratch);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + (rows * a.slots() * 8 + 15) / 16 * 16);
+    const long long blocks = a.pre_blocks + static_cast<long long>(a.groups) * a.size * kv.kv_heads * p.own_tiles * p.own_splits;
+    NNB_ARG_CHECK(blocks <= INT_MAX, "too many queries for one call");
+    if (blocks > 0) {
+        if constexpr (sizeof(T) == 4) {
+            paged_attn_f32_kernel<16><<<static_cast<unsigned>(blocks), 128, 0, s>>>(pool, a);
+            NNB_LAUNCH_CHECK();
+        } else {
+            auto go = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
+                NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
+                kernel<<<static_cast<unsigned>(blocks), 128, bytes, s>>>(pool, a);
+                NNB_LAUNCH_CHECK();
+                return 0;
+            };
+            auto width = [&](auto dp) {
+                constexpr int DP = decltype(dp)::value;
+                static PerDeviceOnce once[3];
+                if (p.rt == 16) return go(paged_attn_bf16_kernel<DP, 1>, AttnTile<DP>::SMEM, once[0]);
+                if (p.rt == 32) return go(paged_attn_bf16_kernel<DP, 2>, AttnTile<DP>::SMEM, once[1]);
+                return go(paged_attn_bf16_kernel<DP, 4>, AttnTile<DP>::SMEM, once[2]);
+            };
+            if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
+            else if (kv.head_dim <= 64) NNB_TRY(width(std::integral_constant<int, 64>()));
+            else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
+            else NNB_TRY(width(std::integral_constant<int, 256>()));
+        }
+    }
+    if (a.slots() == 1) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = blocks > 0 ? 1 : 0;
+    NNB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T>, a, kv.head_dim));
     NNB_LAUNCH_CHECK();
     return 0;
 }
+
 
 static const char* attention_shape_error(const nnb200_paged_kv* kv, int groups, int group_size, int heads, int prefix_stride, int table_stride)
 {
@@ -101,7 +568,9 @@ size_t nnb200_paged_attention_scratch_bytes(const nnb200_paged_kv* kv, int group
         fprintf(stderr, "nnb200: %s: %s\n", __func__, e);
         return 0;
     }
-    return 16;
+    const AttnPlan p = attn_plan(*kv, groups, group_size, heads, prefix_stride, table_stride);
+    const long long slots = static_cast<long long>(groups) * group_size * heads * (p.pre_splits + p.own_splits);
+    return static_cast<size_t>((slots * 8 + 15) / 16 * 16 + slots * kv->head_dim * 4 + 16);
 }
 
 int nnb200_paged_attention(const nnb200_paged_kv* kv, int layer, const void* q, long long ldq, void* out, long long ldo, float* lse,
@@ -119,8 +588,9 @@ int nnb200_paged_attention(const nnb200_paged_kv* kv, int layer, const void* q, 
     NNB_ARG_CHECK(scratch && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "scratch must be there and start on a 16-byte boundary");
     NNB_ARG_CHECK(scratch_bytes >= nnb200_paged_attention_scratch_bytes(kv, groups, group_size, heads, prefix_stride, table_stride), "scratch too small");
     PagedAttnArgs a{q, out, lse, ldq, ldo, prefix_table, prefix_len, page_table, seq_len, prefix_stride, table_stride, groups, group_size, heads, alibi};
-    if (kv->dtype == 0) return attention_t<float>(*kv, layer, a, to_stream(stream));
-    return attention_t<bf16>(*kv, layer, a, to_stream(stream));
+    const AttnPlan p = attn_plan(*kv, groups, group_size, heads, prefix_stride, table_stride);
+    if (kv->dtype == 0) return attention_t<float>(*kv, layer, a, p, scratch, to_stream(stream));
+    return attention_t<bf16>(*kv, layer, a, p, scratch, to_stream(stream));
 }
 
 }  // extern "C"
