@@ -371,58 +371,175 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
     else attend_bf16<DP, 1>(pool, a, k, smem);
 }
 
-// ---------------------------------------------------------------- fp32: a block per task, a warp per cached row in turn
-template <int R>
+// ---------------------------------------------------------------- fp32: FMA tiles
+// Up to 16 query rows against KT cached rows a step.  Scores: a thread takes one cached row and four to eight query rows; softmax:
+// eight lanes a query row; values: a thread takes four columns and every KG-th cached row, for all query rows, and the KG
+// parts are summed at the end.  Rows in shared memory are 16 bytes longer than they are, so that eight neighbours' 16-byte reads
+// meet no bank twice.  fp32 products and sums throughout: infinities and NaN behave as in the formula, which splitting a
+// number into parts for the tensor cores would not keep.
+template <int DP> struct AttnTile32 {
+    static constexpr int KT = DP <= 64 ? 64 : 4096 / DP, LD = DP + 4, CPR = DP / 4, STAGES = 2;
+    static constexpr int G = 128 / KT, RPT = 16 / G;           // sets of query rows, rows of a thread
+    static constexpr int KG = 512 / DP, PL = 20;               // sets of cached rows for the values, row of the weights
+    static constexpr int FLOATS = KT * LD;                     // K, or V, of a stage
+    static constexpr int RING = STAGES * 2 * FLOATS;
+    static constexpr int SMEM = (RING + 16 * DP + KT * PL + 16 * 4) * 4 + STAGES * (KT + 16);
+    static_assert(RING >= 128 * 64, "the join fits the ring");
+    // query row i of set g: fours of rows in turn, so that few rows still spread over the sets
+    static __device__ __forceinline__ int row(int g, int i) { return RPT >= 4 ? (i >> 2) * 4 * G + g * 4 + (i & 3) : g * RPT + i; }
+};
+
+template <int DP>
+__device__ __forceinline__ void load_f32(const PagedPool<float>& pool, const AttnTask& k, uint32_t base, uint8_t* alive, int step, int stage)
+{
+    using Tile = AttnTile32<DP>;
+    const int t0 = k.begin + step * Tile::KT, tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < Tile::KT * Tile::CPR / 128; ++i) {
+        const int idx = tid + i * 128, r = idx / Tile::CPR, c = idx % Tile::CPR, t = t0 + r;
+        int page = -1;
+        if (t < k.end) page = __ldg(k.table + (t >> pool.page_shift));
+        const bool there = page >= 0 && page < pool.pages;
+        const long long off = there && c * 4 < pool.dk ? pool.at(page, k.hk, t & ((1 << pool.page_shift) - 1)) + c * 4 : 0;
+        const int bytes = there && c * 4 < pool.dk ? 16 : 0;
+        const uint32_t dst = base + (stage * 2 * Tile::FLOATS + r * Tile::LD + c * 4) * 4;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pool.k + off), "r"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Tile::FLOATS * 4), "l"(pool.v + off), "r"(bytes) : "memory");
+        if (c == 0) alive[stage * (Tile::KT + 16) + r] = there;
+    }
+}
+
+template <int DP>
 __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> pool, const __grid_constant__ PagedAttnArgs a)
 {
+    extern __shared__ __align__(128) uint8_t smem[];
+    using Tile = AttnTile32<DP>;
+    constexpr int KT = Tile::KT, ST = Tile::STAGES, PL = Tile::PL;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    constexpr int C = 8, WARPS = 4;
-    const AttnTask k = task_of<R>(pool, a, blockIdx.x);
+    const AttnTask k = task_of<16>(pool, a, blockIdx.x);
     if (k.begin >= k.end) { leave_nothing<float>(a, k, pool.dk); return; }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dk = pool.dk, ps = 1 << pool.page_shift;
-    __shared__ float sm[WARPS], sl[WARPS], so[WARPS][256];
-    for (int r = 0; r < k.rows; ++r) {
-        const int seq = seq_of_row(a, k, r), h = head_of_row(a, k, r);
-        const float* qp = static_cast<const float*>(a.q) + seq * a.ldq + static_cast<long long>(h) * dk;
-        float q[C], o[C], m = -INFINITY, l = 0.f;
+    const int tid = threadIdx.x, dk = pool.dk, steps = (k.end - k.begin + KT - 1) / KT;
+    float* ring = reinterpret_cast<float*>(smem);
+    float *sq = ring + Tile::RING, *sp = sq + 16 * DP, *sback = sp + KT * PL, *sslope = sback + 16, *sfar = sslope + 16;
+    uint8_t* alive = reinterpret_cast<uint8_t*>(sfar + 32);
+    const uint32_t base = smem_u32(ring);
 #pragma unroll
-        for (int i = 0; i < C; ++i) { const int c = lane + 32 * i; q[i] = c < dk ? qp[c] : 0.f; o[i] = 0.f; }
-        const float slope = a.alibi ? alibi_slope2(h, a.heads) : 0.f;
-        const int far = far_of(a, pool.page_shift, k, r);
-        for (int t = k.begin + warp; t < k.end; t += WARPS) {
-            const int page = k.table[t >> pool.page_shift];
-            if (page < 0 || page >= pool.pages) continue;
-            const long long at = pool.at(page, k.hk, t & (ps - 1));
-            float s = 0.f, v[C];
+    for (int i = 0; i < ST - 1; ++i) { if (i < steps) load_f32<DP>(pool, k, base, alive, i, i); cp_commit(); }
+    for (int i = tid; i < 16 * DP; i += 128) {
+        const int r = i / DP, c = i - r * DP;
+        sq[i] = r < k.rows && c < dk ? static_cast<const float*>(a.q)[seq_of_row(a, k, r) * a.ldq + static_cast<long long>(head_of_row(a, k, r)) * dk + c] : 0.f;
+    }
+    if (tid < 16) {
+        const bool on = a.alibi && tid < k.rows;
+        sslope[tid] = on ? alibi_slope2(head_of_row(a, k, tid), a.heads) : 0.f;
+        sfar[tid] = on ? static_cast<float>(far_of(a, pool.page_shift, k, tid)) : 0.f;
+    }
+    const int key = tid % KT, set = tid / KT;                   // scores
+    const int srow = tid >> 3, part = tid & 7;                  // softmax
+    const int c4 = tid % (DP / 4), kg = tid / (DP / 4);         // values
+    const int quads = (k.rows + 3) >> 2;
+    float m = -INFINITY, l = 0.f, o[16][4];
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const int c = lane + 32 * i;
-                if (c < dk) s = fmaf(q[i], pool.k[at + c], s);
-                v[i] = c < dk ? pool.v[at + c] : 0.f;
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[r][j] = 0.f;
+
+    for (int step = 0; step < steps; ++step) {
+        cp_wait<ST - 2>();
+        __syncthreads();
+        const int stage = step % ST;
+        if (step + ST - 1 < steps) load_f32<DP>(pool, k, base, alive, step + ST - 1, (step + ST - 1) % ST);
+        cp_commit();
+        const float *sk = ring + stage * 2 * Tile::FLOATS, *sv = sk + Tile::FLOATS;
+        {
+            float s[Tile::RPT];
+#pragma unroll
+            for (int i = 0; i < Tile::RPT; ++i) s[i] = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < DP; d += 4) {
+                const float4 kv = *reinterpret_cast<const float4*>(sk + key * Tile::LD + d);
+#pragma unroll
+                for (int i = 0; i < Tile::RPT; ++i) {
+                    if (Tile::row(set, i) >= k.rows) continue;
+                    const float4 q = *reinterpret_cast<const float4*>(sq + Tile::row(set, i) * DP + d);
+                    s[i] = fmaf(q.x, kv.x, s[i]); s[i] = fmaf(q.y, kv.y, s[i]); s[i] = fmaf(q.z, kv.z, s[i]); s[i] = fmaf(q.w, kv.w, s[i]);
+                }
             }
-            s = warp_sum(s) * a.c - slope * static_cast<float>(far - t);
-            const float nm = fmaxf(m, s), ref = nm == -INFINITY ? 0.f : nm, back = exp2f(m - ref), e = exp2f(s - ref);
-            m = nm;
-            l = l * back + e;
+            const bool there = alive[stage * (KT + 16) + key];
+            const float t = static_cast<float>(k.begin + step * KT + key);
 #pragma unroll
-            for (int i = 0; i < C; ++i) o[i] = fmaf(e, v[i], o[i] * back);
+            for (int i = 0; i < Tile::RPT; ++i) {
+                const int r = Tile::row(set, i);
+                s[i] = there ? s[i] * a.c - sslope[r] * (sfar[r] - t) : -INFINITY;
+            }
+            if constexpr (Tile::RPT >= 4) {
+#pragma unroll
+                for (int i = 0; i < Tile::RPT; i += 4) *reinterpret_cast<float4*>(sp + key * PL + Tile::row(set, i)) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < Tile::RPT; ++i) sp[key * PL + Tile::row(set, i)] = s[i];
+            }
         }
         __syncthreads();
-        if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+        float s[KT / 8], top = m;
 #pragma unroll
-        for (int i = 0; i < C; ++i) so[warp][lane + 32 * i] = o[i];
-        __syncthreads();
-        for (int c = threadIdx.x * 4; c < dk; c += 512) {
-            float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), sum = 0.f;
-            const float ref = top == -INFINITY ? 0.f : top;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < WARPS; ++w) {
-                const float e = exp2f(sm[w] - ref);
-                sum = fmaf(sl[w], e, sum);
-                x.x = fmaf(so[w][c], e, x.x); x.y = fmaf(so[w][c + 1], e, x.y); x.z = fmaf(so[w][c + 2], e, x.z); x.w = fmaf(so[w][c + 3], e, x.w);
-            }
-            leave<float>(a, k, dk, r, c, x, top, sum);
+        for (int j = 0; j < KT / 8; ++j) { s[j] = sp[(part + 8 * j) * PL + srow]; top = fmaxf(top, s[j]); }
+#pragma unroll
+        for (int w = 1; w < 8; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        const float ref = top == -INFINITY ? 0.f : top, back = exp2f(m - ref);
+        const bool moved = top != m;
+        l *= back;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j) {
+            s[j] = exp2f(s[j] - ref);
+            l += s[j];
+            sp[(part + 8 * j) * PL + srow] = s[j];
         }
+        if (part == 0) sback[srow] = back;
+        if (__syncthreads_or(moved)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float b = sback[r];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[r][j] *= b;
+            }
+        }
+#pragma unroll 2
+        for (int t = kg; t < KT; t += Tile::KG) {
+            const float4 v = *reinterpret_cast<const float4*>(sv + t * Tile::LD + c4 * 4);
+#pragma unroll
+            for (int rq = 0; rq < 4; ++rq) {
+                if (rq >= quads) break;
+                const float4 p = *reinterpret_cast<const float4*>(sp + t * PL + rq * 4);
+                const float pr[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float* x = o[rq * 4 + i];
+                    x[0] = fmaf(pr[i], v.x, x[0]); x[1] = fmaf(pr[i], v.y, x[1]); x[2] = fmaf(pr[i], v.z, x[2]); x[3] = fmaf(pr[i], v.w, x[3]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int w = 1; w < 8; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    cp_wait<0>();
+    __syncthreads();
+    if (part == 0) { sslope[srow] = m; sfar[srow] = l; }
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (r < k.rows) *reinterpret_cast<float4*>(ring + (kg * 16 + r) * DP + c4 * 4) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+    __syncthreads();
+    const int vecs = dk / 4;
+    for (int idx = tid; idx < k.rows * vecs; idx += 128) {
+        const int r = idx / vecs, c = (idx - r * vecs) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < Tile::KG; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(ring + (w * 16 + r) * DP + c);
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+        leave<float>(a, k, dk, r, c, x, sslope[r], sfar[r]);
     }
 }
 
@@ -507,28 +624,26 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
     const long long blocks = a.pre_blocks + static_cast<long long>(a.groups) * a.size * kv.kv_heads * p.own_tiles * p.own_splits;
     NNB_ARG_CHECK(blocks <= INT_MAX, "too many queries for one call");
     if (blocks > 0) {
-        if constexpr (sizeof(T) == 4) {
-            paged_attn_f32_kernel<16><<<static_cast<unsigned>(blocks), 128, 0, s>>>(pool, a);
+        auto go = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
+            NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
+            kernel<<<static_cast<unsigned>(blocks), 128, bytes, s>>>(pool, a);
             NNB_LAUNCH_CHECK();
-        } else {
-            auto go = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
-                NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
-                kernel<<<static_cast<unsigned>(blocks), 128, bytes, s>>>(pool, a);
-                NNB_LAUNCH_CHECK();
-                return 0;
-            };
-            auto width = [&](auto dp) {
-                constexpr int DP = decltype(dp)::value;
-                static PerDeviceOnce once[3];
+            return 0;
+        };
+        auto width = [&](auto dp) {
+            constexpr int DP = decltype(dp)::value;
+            static PerDeviceOnce once[3];
+            if constexpr (sizeof(T) == 4) return go(paged_attn_f32_kernel<DP>, AttnTile32<DP>::SMEM, once[0]);
+            else {
                 if (p.rt == 16) return go(paged_attn_bf16_kernel<DP, 1>, AttnTile<DP>::SMEM, once[0]);
                 if (p.rt == 32) return go(paged_attn_bf16_kernel<DP, 2>, AttnTile<DP>::SMEM, once[1]);
                 return go(paged_attn_bf16_kernel<DP, 4>, AttnTile<DP>::SMEM, once[2]);
-            };
-            if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
-            else if (kv.head_dim <= 64) NNB_TRY(width(std::integral_constant<int, 64>()));
-            else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
-            else NNB_TRY(width(std::integral_constant<int, 256>()));
-        }
+            }
+        };
+        if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
+        else if (kv.head_dim <= 64) NNB_TRY(width(std::integral_constant<int, 64>()));
+        else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
+        else NNB_TRY(width(std::integral_constant<int, 256>()));
     }
     if (a.slots() == 1) return 0;
     cudaLaunchConfig_t cfg = {};
