@@ -23,15 +23,17 @@ struct PagedAttnArgs {
     long long ldq, ldo;
     const int *prefix_table, *prefix_len, *table, *len;
     int prefix_stride, table_stride, groups, size, heads, alibi;
-    int m;                          // query heads per cached head
-    int row_tiles, own_tiles;       // tiles of a group's rows, of a sequence's
-    int pre_splits, own_splits;     // blocks that share a prefix, a sequence's own rows
-    long long pre_blocks;           // blocks [0, pre_blocks) take prefixes, the others own rows
+    FastDiv m;                      // query heads per cached head
+    FastDiv row_tiles, own_tiles;   // tiles of a group's rows, of a sequence's
+    FastDiv pre_splits, own_splits; // blocks that share a prefix, a sequence's own rows (0: divisor 1, and no task)
+    FastDiv by_size, by_kv_heads, by_vecs, by_heads;
+    int slots, pre_slots, own_rows; // places of a query row's partial results, the prefix's among them; rows of an own tile
+    int own_warps;                  // warps that share a task of own rows: 4, or 1 (four tasks in a block)
+    int pre_blocks, tasks;          // tasks [0, pre_blocks) are prefixes, a block each; the others own rows
     int pairs;                      // queries may be read two columns at a time
     float c;                        // log2(e) / sqrt(head_dim): exponentials are powers of two
     float* part;                    // (query row, slot): head_dim sums
     float2* stat;                   // (query row, slot): maximum (in powers of two) and sum; sum 0: nothing there
-    __host__ __device__ int slots() const { return pre_splits + own_splits; }
 };
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -61,43 +63,47 @@ __device__ __forceinline__ void share_of(int len, int splits, int s, int& begin,
     end = min(len - begin, per) + begin;
 }
 template <int RT, typename T>
-__device__ __forceinline__ AttnTask task_of(const PagedPool<T>& pool, const PagedAttnArgs& a, long long b)
+__device__ __forceinline__ AttnTask task_of(const PagedPool<T>& pool, const PagedAttnArgs& a, int b)
 {
     AttnTask k;
     if (b < a.pre_blocks) {                                     // neighbours share their cached rows: row tiles, then splits
-        const int rt = static_cast<int>(b % a.row_tiles); b /= a.row_tiles;
-        const int s = static_cast<int>(b % a.pre_splits); b /= a.pre_splits;
-        k.hk = static_cast<int>(b % pool.kv_heads);
-        const int g = static_cast<int>(b / pool.kv_heads);
+        int rest = a.row_tiles.split(b);                        // b: row tile
+        int head = a.pre_splits.split(rest);                    // rest: split
+        const int g = a.by_kv_heads.split(head);
+        k.hk = head;
         k.group = g;
-        k.first = rt * RT;
-        k.rows = min(a.size * a.m - k.first, RT);
+        k.first = b * RT;
+        k.rows = min(a.size * static_cast<int>(a.m.d) - k.first, RT);
         k.table = a.prefix_table + static_cast<long long>(g) * a.prefix_stride;
         k.place = 0;
-        k.slot = s;
-        share_of(held(a.prefix_len[g], a.prefix_stride, pool.page_shift), a.pre_splits, s, k.begin, k.end);
+        k.slot = rest;
+        share_of(held(a.prefix_len[g], a.prefix_stride, pool.page_shift), a.pre_slots, rest, k.begin, k.end);
         return k;
     }
     b -= a.pre_blocks;
-    const int rt = static_cast<int>(b % a.own_tiles); b /= a.own_tiles;
-    const int s = static_cast<int>(b % a.own_splits); b /= a.own_splits;
-    k.hk = static_cast<int>(b % pool.kv_heads);
-    const int seq = static_cast<int>(b / pool.kv_heads);
-    k.group = seq / a.size;
-    k.first = (seq - k.group * a.size) * a.m + rt * 16;
-    k.rows = min(a.m - rt * 16, 16);
+    int rest = a.own_tiles.split(b), head = a.own_splits.split(rest);
+    const int seq = a.by_kv_heads.split(head), m = static_cast<int>(a.m.d);
+    k.hk = head;
+    k.group = a.by_size.div(seq);
+    k.first = (seq - k.group * a.size) * m + b * a.own_rows;
+    k.rows = min(m - b * a.own_rows, a.own_rows);
     k.table = a.table + static_cast<long long>(seq) * a.table_stride;
     k.place = a.prefix_stride ? held(a.prefix_len[k.group], a.prefix_stride, pool.page_shift) : 0;
-    k.slot = a.pre_splits + s;
-    share_of(held(a.len[seq], a.table_stride, pool.page_shift), a.own_splits, s, k.begin, k.end);
+    k.slot = a.pre_slots + rest;
+    share_of(held(a.len[seq], a.table_stride, pool.page_shift), static_cast<int>(a.own_splits.d), rest, k.begin, k.end);
     return k;
 }
-__device__ __forceinline__ int seq_of_row(const PagedAttnArgs& a, const AttnTask& k, int r) { return k.group * a.size + (k.first + r) / a.m; }
-__device__ __forceinline__ int head_of_row(const PagedAttnArgs& a, const AttnTask& k, int r) { return k.hk * a.m + (k.first + r) % a.m; }
-// distance from row `place + t` to the last one the query sees is far_of - t
-__device__ __forceinline__ int far_of(const PagedAttnArgs& a, int shift, const AttnTask& k, int r)
+// query row r of a task
+struct AttnRow { int seq, head; };
+__device__ __forceinline__ AttnRow row_of(const PagedAttnArgs& a, const AttnTask& k, int r)
 {
-    const int seq = seq_of_row(a, k, r);
+    int j = k.first + r;
+    const int i = a.m.split(j);
+    return {k.group * a.size + i, k.hk * static_cast<int>(a.m.d) + j};
+}
+// distance from row `place + t` to the last one the query sees is far_of - t
+__device__ __forceinline__ int far_of(const PagedAttnArgs& a, int shift, const AttnTask& k, int seq)
+{
     const int pre = a.prefix_stride ? held(a.prefix_len[k.group], a.prefix_stride, shift) : 0;
     return pre + (a.table_stride ? held(a.len[seq], a.table_stride, shift) : 0) - 1 - k.place;
 }
@@ -131,10 +137,9 @@ template <int DP> struct AttnLoader {
 #pragma unroll
         for (int i = 0; i < Tile::KT * Tile::CPR / 128; ++i) {
             const int idx = tid + i * 128, r = idx / Tile::CPR, c = idx % Tile::CPR, t = t0 + r;
-            int page = -1;
-            if (t < k.end) page = __ldg(k.table + (t >> pool.page_shift));
-            const bool there = page >= 0 && page < pool.pages;
-            const long long off = there && c * 8 < pool.dk ? pool.at(page, k.hk, t & ((1 << pool.page_shift) - 1)) + c * 8 : 0;
+            const int row = t < k.end ? pool.find(k.table, k.hk, t) : -1;
+            const bool there = row >= 0;
+            const long long off = there && c * 8 < pool.dk ? static_cast<long long>(row) * pool.dk + c * 8 : 0;
             const int bytes = there && c * 8 < pool.dk ? 16 : 0;
             const uint32_t dst = base + stage * 2 * Tile::BYTES + Tile::at(r, c);
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pool.k + off), "r"(bytes) : "memory");
@@ -168,27 +173,27 @@ __device__ __forceinline__ bool sees(const PagedAttnArgs& a, int seq) { return a
 template <typename T>
 __device__ __forceinline__ void leave(const PagedAttnArgs& a, const AttnTask& k, int dk, int r, int c, float4 o, float m, float l)
 {
-    const int seq = seq_of_row(a, k, r), h = head_of_row(a, k, r);
-    const long long row = static_cast<long long>(seq) * a.heads + h;
-    if (a.slots() == 1) {
-        const bool none = l == 0.f || !sees(a, seq);
-        T* to = static_cast<T*>(a.out) + seq * a.ldo + static_cast<long long>(h) * dk + c;
+    const AttnRow w = row_of(a, k, r);
+    const long long row = static_cast<long long>(w.seq) * a.heads + w.head;
+    if (a.slots == 1) {
+        const bool none = l == 0.f || !sees(a, w.seq);
+        T* to = static_cast<T*>(a.out) + w.seq * a.ldo + static_cast<long long>(w.head) * dk + c;
         const float inv = none ? 0.f : 1.0f / l;
         to[0] = from_f32<T>(none ? 0.f : o.x * inv); to[1] = from_f32<T>(none ? 0.f : o.y * inv);
         to[2] = from_f32<T>(none ? 0.f : o.z * inv); to[3] = from_f32<T>(none ? 0.f : o.w * inv);
         if (c == 0 && a.lse) a.lse[row] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         return;
     }
-    const long long at = row * a.slots() + k.slot;
+    const long long at = row * a.slots + k.slot;
     *reinterpret_cast<float4*>(a.part + at * dk + c) = o;
     if (c == 0) a.stat[at] = make_float2(m, l);
 }
 template <typename T>
-__device__ __forceinline__ void leave_nothing(const PagedAttnArgs& a, const AttnTask& k, int dk)
+__device__ __forceinline__ void leave_nothing(const PagedAttnArgs& a, const AttnTask& k, int dk, int first, int stride)
 {
-    for (int r = threadIdx.x; r < k.rows; r += blockDim.x) {
-        const int seq = seq_of_row(a, k, r), h = head_of_row(a, k, r);
-        if (a.slots() > 1) a.stat[(static_cast<long long>(seq) * a.heads + h) * a.slots() + k.slot] = make_float2(-INFINITY, 0.f);
+    for (int r = first; r < k.rows; r += stride) {
+        const AttnRow w = row_of(a, k, r);
+        if (a.slots > 1) a.stat[(static_cast<long long>(w.seq) * a.heads + w.head) * a.slots + k.slot] = make_float2(-INFINITY, 0.f);
         else for (int c = 0; c < dk; c += 4) leave<T>(a, k, dk, r, c, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
     }
 }
@@ -214,9 +219,9 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
         const bool live = r < k.rows;
         const bf16* q = static_cast<const bf16*>(a.q);
         if (live) {
-            const int h = head_of_row(a, k, r);
-            q += seq_of_row(a, k, r) * a.ldq + static_cast<long long>(h) * dk;
-            if (a.alibi) { slope[i] = alibi_slope2(h, a.heads); far[i] = static_cast<float>(far_of(a, pool.page_shift, k, r)); }
+            const AttnRow w = row_of(a, k, r);
+            q += w.seq * a.ldq + static_cast<long long>(w.head) * dk;
+            if (a.alibi) { slope[i] = alibi_slope2(w.head, a.heads); far[i] = static_cast<float>(far_of(a, pool.page_shift, k, w.seq)); }
         }
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
@@ -232,6 +237,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
             }
     }
 
+    const float mul = a.alibi ? 1.f : a.c;                      // scores are scaled inside the exponent, or with the bias before it
     float o[ND][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < ND; ++n)
@@ -261,13 +267,12 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
                 mma_bf16(s[n + 1], qf[kk], b[2], b[3]);
             }
         const int t0 = k.begin + step * Tile::KT + key0 + (lane & 3) * 2;
+        if (a.alibi) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[n][j] *= a.c;
-                if (a.alibi) s[n][j] -= slope[j >> 1] * (far[j >> 1] - static_cast<float>(t0 + n * 8 + (j & 1)));
-            }
+                for (int j = 0; j < 4; ++j) s[n][j] = s[n][j] * a.c - slope[j >> 1] * (far[j >> 1] - static_cast<float>(t0 + n * 8 + (j & 1)));
+        }
         const uint8_t* al = alive + stage * (Tile::KT + 16);
         if (*reinterpret_cast<const uint32_t*>(al + Tile::KT)) {
 #pragma unroll
@@ -276,7 +281,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
                 for (int j = 0; j < 2; ++j)
                     if (!al[key0 + n * 8 + (lane & 3) * 2 + j]) { s[n][j] = -INFINITY; s[n][j + 2] = -INFINITY; }
         }
-        float top[2] = {m[0], m[1]};
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
@@ -286,6 +291,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
         for (int i = 0; i < 2; ++i) {
             top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
             top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+            top[i] = fmaxf(m[i], top[i] * mul);
         }
         float ref[2];
 #pragma unroll
@@ -303,7 +309,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { s[n][j] = exp2_fast(s[n][j] - ref[j >> 1]); l[j >> 1] += s[n][j]; }
+            for (int j = 0; j < 4; ++j) { s[n][j] = exp2_fast(fmaf(s[n][j], mul, -ref[j >> 1])); l[j >> 1] += s[n][j]; }
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
             // the weights are rounded to bf16 for the tensor cores (their sum is not): 2^-9 of a weight, what rounding V costs too
@@ -341,7 +347,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
     __syncthreads();
     const int vecs = dk / 4;
     for (int idx = threadIdx.x; idx < k.rows * vecs; idx += 128) {
-        const int r = idx / vecs, c = (idx - r * vecs) * 4, w0 = (r >> 4) * WK, rr = r & 15;
+        const int r = a.by_vecs.div(idx), c = (idx - r * vecs) * 4, w0 = (r >> 4) * WK, rr = r & 15;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < WK; ++w) top = fmaxf(top, sml[(w0 + w) * 16 + rr].x);
@@ -360,15 +366,279 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
     }
 }
 
-template <int DP, int WM>
+// Up to 16 query rows: nothing is shared between warps, so each warp streams cached rows through a ring of its own, KW rows a
+// step, without a barrier, and the WT warps of a task (one, or the block's four) take its steps in turn and are joined at the
+// end.  The products are transposed, S' = K Q' and O' = V' P', so that cached rows fill the 16 rows of a tensor core tile and
+// queries its 8 columns (NQ = 1 or 2 of them): one query costs half of what it would as one of 16 rows.  P' comes out of the
+// first product with cached rows down and queries across; the second wants it the other way round, an 8 x 8 transposition.
+// A lane looks up one cached row of a step, a step before it is copied; the copies get it by shuffle.  Rows in shared memory
+// are 16 bytes longer than they are: eight neighbours at one column meet no bank twice.  The reference point of the exponentials
+// moves only when a score is more than 2^8 above it: scores then need no maximum across lanes.
+template <int DP> struct AttnStream {
+    static constexpr int KW = DP <= 32 ? 32 : 16, ST = DP <= 64 ? 3 : 2, PITCH = DP * 2 + 16, CPR = DP / 8;
+    static constexpr int PLANE = KW * PITCH, STAGE = 2 * PLANE, RING = ST * STAGE;
+    static constexpr int SMEM = 4 * (RING + 16);
+};
+// what a score may be above the reference point of its row's exponentials, in powers of two: sums stay far from overflow
+constexpr float kAttnSlack = 8.0f;
+
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <int DP, int NQ>
+__device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const PagedAttnArgs& a, const AttnTask& k, uint8_t* smem, int wt)
+{
+    using Str = AttnStream<DP>;
+    constexpr int KW = Str::KW, NK = KW / 16, ND = DP / 16, KS = DP / 16, ST = Str::ST, CPR = Str::CPR;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wk = wt == 1 ? 0 : warp, dk = pool.dk;
+    const int all = (k.end - k.begin + KW - 1) / KW, steps = (all - wk + wt - 1) / wt;
+    const uint32_t ring = smem_u32(smem) + warp * Str::RING;
+    uint32_t* alive = reinterpret_cast<uint32_t*>(smem + 4 * Str::RING) + warp * 4;
+    // the cached row this lane looks up for a step (lanes beyond KW: none)
+    auto look = [&](int step) {
+        const int t = k.begin + (step * wt + wk) * KW + lane;
+        return step < steps && lane < KW && t < k.end ? pool.find(k.table, k.hk, t) : -1;
+    };
+    // lane l copies chunk l % CPR of rows l / CPR, l / CPR + RPI, ..
+    constexpr int RPI = 32 / CPR;                               // rows the warp copies at once
+    const int chunk = lane % CPR;
+    const bool in = chunk * 8 < dk;
+    const char* kbase = reinterpret_cast<const char*>(pool.k + (in ? chunk * 8 : 0));
+    const char* vbase = reinterpret_cast<const char*>(pool.v + (in ? chunk * 8 : 0));
+    const uint32_t dst0 = ring + (lane / CPR) * Str::PITCH + chunk * 16;
+    auto fetch = [&](int row, int stage) {
+        const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
+        if (lane == 0) alive[stage] = mask;
+#pragma unroll
+        for (int i = 0; i < KW / RPI; ++i) {
+            const int r = __shfl_sync(0xffffffffu, row, i * RPI + lane / CPR);
+            const long long off = static_cast<long long>(max(r, 0)) * (dk * 2);
+            const int bytes = r >= 0 && in ? 16 : 0;
+            const uint32_t dst = dst0 + stage * Str::STAGE + i * RPI * Str::PITCH;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(kbase + off), "r"(bytes) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Str::PLANE), "l"(vbase + off), "r"(bytes) : "memory");
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) { const int row = look(i); if (i < steps) fetch(row, i); cp_commit(); }
+    int next = look(ST - 1);
+
+    const int g = lane >> 2, t2 = (lane & 3) * 2;               // queries as columns: g for loading them, t2 and t2 + 1 in the products
+    uint32_t qf[NQ][KS][2];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = n * 8 + g;
+        const bool live = r < k.rows;
+        const AttnRow w = row_of(a, k, live ? r : 0);
+        const bf16* q = static_cast<const bf16*>(a.q) + w.seq * a.ldq + static_cast<long long>(w.head) * dk + t2;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c = kk * 16 + j * 8;
+                uint32_t v = 0;
+                if (live && c + t2 < dk) {
+                    if (a.pairs) v = *reinterpret_cast<const uint32_t*>(q + c);
+                    else v = static_cast<uint32_t>(__bfloat16_as_ushort(q[c])) | static_cast<uint32_t>(__bfloat16_as_ushort(q[c + 1])) << 16;
+                }
+                qf[n][kk][j] = v;
+            }
+    }
+    float slope[NQ][2], far[NQ][2], m[NQ][2], l[NQ][2], o[ND][NQ][4];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            slope[n][i] = 0.f; far[n][i] = 0.f; m[n][i] = -INFINITY; l[n][i] = 0.f;
+            if (a.alibi && n * 8 + t2 + i < k.rows) {
+                const AttnRow w = row_of(a, k, n * 8 + t2 + i);
+                slope[n][i] = alibi_slope2(w.head, a.heads);
+                far[n][i] = static_cast<float>(far_of(a, pool.page_shift, k, w.seq));
+            }
+        }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[d][n][j] = 0.f;
+    const float mul = a.alibi ? 1.f : a.c;                      // scores are scaled inside the exponent, or with the bias before it
+
+    int stage = 0;
+    for (int step = 0; step < steps; ++step) {
+        cp_wait<ST - 2>();
+        __syncwarp();
+        if (step + ST - 1 < steps) fetch(next, stage == 0 ? ST - 1 : stage - 1);
+        cp_commit();
+        next = look(step + ST);
+        const uint32_t kb = ring + stage * Str::STAGE + ((lane & 7) + ((lane >> 3) & 1) * 8) * Str::PITCH + (lane >> 4) * 16;
+        const uint32_t vb = ring + stage * Str::STAGE + Str::PLANE + ((lane & 7) + (lane >> 4) * 8) * Str::PITCH + ((lane >> 3) & 1) * 16;
+        const uint32_t mask = alive[stage];
+        stage = stage == ST - 1 ? 0 : stage + 1;
+        float s[NK][NQ][4];                                     // cached row g (0, 1) or g + 8 (2, 3), query t2 (0, 2) or t2 + 1 (1, 3)
+#pragma unroll
+        for (int x = 0; x < NK; ++x) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[x][n][j] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                uint32_t f[4];
+                ldsm4(f, kb + x * 16 * Str::PITCH + kk * 32);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) mma_bf16(s[x][n], f, qf[n][kk][0], qf[n][kk][1]);
+            }
+        }
+        if (a.alibi) {
+            const float t0 = static_cast<float>(k.begin + (step * wt + wk) * KW + g);
+#pragma unroll
+            for (int x = 0; x < NK; ++x)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[x][n][j] = s[x][n][j] * a.c - slope[n][j & 1] * (far[n][j & 1] - (t0 + static_cast<float>(x * 16 + (j >> 1) * 8)));
+        }
+        if (mask != (KW == 32 ? 0xffffffffu : (1u << (KW & 31)) - 1u)) {
+#pragma unroll
+            for (int x = 0; x < NK; ++x)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (!(mask >> (x * 16 + g + i * 8) & 1u)) {
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n) { s[x][n][2 * i] = -INFINITY; s[x][n][2 * i + 1] = -INFINITY; }
+                    }
+        }
+        bool ahead = false;
+        float top[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                top[n][i] = fmaxf(s[0][n][i], s[0][n][i + 2]);
+#pragma unroll
+                for (int x = 1; x < NK; ++x) top[n][i] = fmaxf(top[n][i], fmaxf(s[x][n][i], s[x][n][i + 2]));
+                top[n][i] *= mul;
+                ahead |= top[n][i] > m[n][i] + kAttnSlack;
+            }
+        if (__any_sync(0xffffffffu, ahead)) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float x = top[n][i];
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+                    x = fmaxf(x, m[n][i]);
+                    const float back = exp2_fast(m[n][i] - (x == -INFINITY ? 0.f : x));
+                    m[n][i] = x;
+                    l[n][i] *= back;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) { o[d][n][i] *= back; o[d][n][i + 2] *= back; }
+                }
+        }
+        float ref[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) ref[n][i] = m[n][i] == -INFINITY ? 0.f : m[n][i];
+#pragma unroll
+        for (int x = 0; x < NK; ++x) {
+            uint32_t p[NQ][2];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float e[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { e[j] = exp2_fast(fmaf(s[x][n][j], mul, -ref[n][j & 1])); l[n][j & 1] += e[j]; }
+                // the weights are rounded to bf16 for the tensor cores (their sum is not): half a step of 2^-8, what rounding V costs too
+                p[n][0] = transposed8x8(pack_bf16x2(e[0], e[1]));
+                p[n][1] = transposed8x8(pack_bf16x2(e[2], e[3]));
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                uint32_t f[4];
+                ldsm4_t(f, vb + x * 16 * Str::PITCH + d * 32);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) mma_bf16(o[d][n], f, p[n][0], p[n][1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], w);
+    cp_wait<0>();
+    if (wt == 1) __syncwarp();
+    else __syncthreads();
+    // through shared memory, so that rows are written with whole vectors; the warps of a task are joined on the way
+    constexpr int LD = DP + 4;
+    static_assert(NQ * 8 * (LD * 4 + 8) <= Str::RING, "the join fits a warp's ring");
+    float* so = reinterpret_cast<float*>(smem + warp * Str::RING);
+    float2* sml = reinterpret_cast<float2*>(so + NQ * 8 * LD);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = n * 8 + t2 + i;
+            if (r < k.rows) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) { so[r * LD + d * 16 + g] = o[d][n][i]; so[r * LD + d * 16 + g + 8] = o[d][n][i + 2]; }
+                if (g == 0) sml[r] = make_float2(m[n][i], l[n][i]);
+            }
+        }
+    if (wt == 1) __syncwarp();
+    else __syncthreads();
+    const int vecs = dk / 4;
+    for (int idx = wt == 1 ? lane : threadIdx.x; idx < k.rows * vecs; idx += 32 * wt) {
+        const int r = a.by_vecs.div(idx), c = (idx - r * vecs) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, sum = 0.f;
+        if (wt == 1) {
+            x = *reinterpret_cast<const float4*>(so + r * LD + c);
+            top = sml[r].x; sum = sml[r].y;
+        } else {
+            const float* s0 = reinterpret_cast<const float*>(smem);
+            float2 st[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) { st[w] = *reinterpret_cast<const float2*>(s0 + w * (Str::RING / 4) + NQ * 8 * LD + 2 * r); top = fmaxf(top, st[w].x); }
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float e = exp2_fast(st[w].x - ref);
+                const float4 y = *reinterpret_cast<const float4*>(s0 + w * (Str::RING / 4) + r * LD + c);
+                sum = fmaf(st[w].y, e, sum);
+                x.x = fmaf(y.x, e, x.x); x.y = fmaf(y.y, e, x.y); x.z = fmaf(y.z, e, x.z); x.w = fmaf(y.w, e, x.w);
+            }
+        }
+        leave<bf16>(a, k, dk, r, c, x, top, sum);
+    }
+}
+
+template <int DP, int WM, int NQ>
 __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const AttnTask k = task_of<WM * 16>(pool, a, blockIdx.x);
-    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk); return; }
-    if (blockIdx.x < a.pre_blocks) attend_bf16<DP, WM>(pool, a, k, smem);
-    else attend_bf16<DP, 1>(pool, a, k, smem);
+    const int b = static_cast<int>(blockIdx.x);
+    if (b < a.pre_blocks) {
+        const AttnTask k = task_of<WM == 1 ? NQ * 8 : WM * 16>(pool, a, b);
+        if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 128); return; }
+        if constexpr (WM == 1) stream_bf16<DP, NQ>(pool, a, k, smem, 4);
+        else attend_bf16<DP, WM>(pool, a, k, smem);
+        return;
+    }
+    // own rows: a task for the block, or one for each of its warps
+    const int task = a.own_warps == 4 ? b : a.pre_blocks + (b - a.pre_blocks) * 4 + static_cast<int>(threadIdx.x >> 5);
+    if (task >= a.tasks) return;
+    const AttnTask k = task_of<WM == 1 ? NQ * 8 : WM * 16>(pool, a, task);
+    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, a.own_warps == 4 ? threadIdx.x : threadIdx.x & 31, 32 * a.own_warps); return; }
+    stream_bf16<DP, NQ>(pool, a, k, smem, a.own_warps);
 }
 
 // ---------------------------------------------------------------- fp32: FMA tiles
@@ -397,10 +667,9 @@ __device__ __forceinline__ void load_f32(const PagedPool<float>& pool, const Att
 #pragma unroll
     for (int i = 0; i < Tile::KT * Tile::CPR / 128; ++i) {
         const int idx = tid + i * 128, r = idx / Tile::CPR, c = idx % Tile::CPR, t = t0 + r;
-        int page = -1;
-        if (t < k.end) page = __ldg(k.table + (t >> pool.page_shift));
-        const bool there = page >= 0 && page < pool.pages;
-        const long long off = there && c * 4 < pool.dk ? pool.at(page, k.hk, t & ((1 << pool.page_shift) - 1)) + c * 4 : 0;
+        const int row = t < k.end ? pool.find(k.table, k.hk, t) : -1;
+        const bool there = row >= 0;
+        const long long off = there && c * 4 < pool.dk ? static_cast<long long>(row) * pool.dk + c * 4 : 0;
         const int bytes = there && c * 4 < pool.dk ? 16 : 0;
         const uint32_t dst = base + (stage * 2 * Tile::FLOATS + r * Tile::LD + c * 4) * 4;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pool.k + off), "r"(bytes) : "memory");
@@ -417,7 +686,7 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
     constexpr int KT = Tile::KT, ST = Tile::STAGES, PL = Tile::PL;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const AttnTask k = task_of<16>(pool, a, blockIdx.x);
-    if (k.begin >= k.end) { leave_nothing<float>(a, k, pool.dk); return; }
+    if (k.begin >= k.end) { leave_nothing<float>(a, k, pool.dk, threadIdx.x, 128); return; }
     const int tid = threadIdx.x, dk = pool.dk, steps = (k.end - k.begin + KT - 1) / KT;
     float* ring = reinterpret_cast<float*>(smem);
     float *sq = ring + Tile::RING, *sp = sq + 16 * DP, *sback = sp + KT * PL, *sslope = sback + 16, *sfar = sslope + 16;
@@ -427,12 +696,14 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
     for (int i = 0; i < ST - 1; ++i) { if (i < steps) load_f32<DP>(pool, k, base, alive, i, i); cp_commit(); }
     for (int i = tid; i < 16 * DP; i += 128) {
         const int r = i / DP, c = i - r * DP;
-        sq[i] = r < k.rows && c < dk ? static_cast<const float*>(a.q)[seq_of_row(a, k, r) * a.ldq + static_cast<long long>(head_of_row(a, k, r)) * dk + c] : 0.f;
+        const AttnRow w = row_of(a, k, r);
+        sq[i] = r < k.rows && c < dk ? static_cast<const float*>(a.q)[w.seq * a.ldq + static_cast<long long>(w.head) * dk + c] : 0.f;
     }
     if (tid < 16) {
         const bool on = a.alibi && tid < k.rows;
-        sslope[tid] = on ? alibi_slope2(head_of_row(a, k, tid), a.heads) : 0.f;
-        sfar[tid] = on ? static_cast<float>(far_of(a, pool.page_shift, k, tid)) : 0.f;
+        const AttnRow w = row_of(a, k, on ? tid : 0);
+        sslope[tid] = on ? alibi_slope2(w.head, a.heads) : 0.f;
+        sfar[tid] = on ? static_cast<float>(far_of(a, pool.page_shift, k, w.seq)) : 0.f;
     }
     const int key = tid % KT, set = tid / KT;                   // scores
     const int srow = tid >> 3, part = tid & 7;                  // softmax
@@ -532,7 +803,7 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
     __syncthreads();
     const int vecs = dk / 4;
     for (int idx = tid; idx < k.rows * vecs; idx += 128) {
-        const int r = idx / vecs, c = (idx - r * vecs) * 4;
+        const int r = a.by_vecs.div(idx), c = (idx - r * vecs) * 4;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < Tile::KG; ++w) {
@@ -550,7 +821,8 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 {
     __shared__ float sx[128 * 4], sl[128], red[32];
     const long long row = blockIdx.x;
-    const int seq = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<long long>(seq) * a.heads), slots = a.slots();
+    int h = static_cast<int>(blockIdx.x);
+    const int seq = a.by_heads.split(h), slots = a.slots;
     const bool live = sees(a, seq);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const float2* st = a.stat + row * slots;
@@ -558,7 +830,7 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
     for (int i = threadIdx.x; i < slots; i += 128) m = fmaxf(m, st[i].x);
     m = block_max(m, red);
     const float ref = m == -INFINITY ? 0.f : m;
-    const int vecs = dk / 4, sets = 128 / vecs, set = threadIdx.x / vecs, c = (threadIdx.x - set * vecs) * 4;
+    const int vecs = dk / 4, sets = a.by_vecs.div(128), set = a.by_vecs.div(threadIdx.x), c = (threadIdx.x - set * vecs) * 4;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
     if (set < sets)
@@ -589,15 +861,17 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------- how the work is cut
-struct AttnPlan { int rt, row_tiles, own_tiles, pre_splits, own_splits; };
+struct AttnPlan { int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps; };
 static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int heads, int prefix_stride, int table_stride)
 {
     AttnPlan p;
     const int m = heads / kv.kv_heads;
     const long long rows = static_cast<long long>(size) * m;
-    p.rt = rows <= 16 || kv.dtype == 0 ? 16 : (rows <= 32 ? 32 : 64);
+    // fp32 tiles take 16 query rows; bf16 streams 8 or 16, the shared tiles 32 or 64
+    p.rt = kv.dtype == 0 ? 16 : (rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 64)));
+    p.own_rows = kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16)) ? 8 : 16;
     p.row_tiles = static_cast<int>(ceil_div(rows, p.rt));
-    p.own_tiles = (m + 15) / 16;
+    p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
     const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
     const long long pre_units = static_cast<long long>(groups) * kv.kv_heads * p.row_tiles, own_units = static_cast<long long>(groups) * size * kv.kv_heads * p.own_tiles;
     // cached rows for a block when the tables are full: enough blocks for the machine a few times over, at least two steps each
@@ -606,6 +880,7 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     chunk = std::min<long long>(std::max<long long>(ceil_div(chunk, 64) * 64, 128), 1 << 20);
     p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
     p.own_splits = static_cast<int>(ceil_div(own, chunk));
+    p.own_warps = kv.dtype == 0 || ceil_div(own, std::max(1, p.own_splits)) > 512 ? 4 : 1;
     return p;
 }
 
@@ -614,15 +889,20 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
 {
     const PagedPool<T> pool = paged_pool<T>(kv, layer);
     const long long rows = static_cast<long long>(a.groups) * a.size * a.heads;
-    a.m = a.heads / kv.kv_heads;
-    a.row_tiles = p.row_tiles; a.own_tiles = p.own_tiles; a.pre_splits = p.pre_splits; a.own_splits = p.own_splits;
-    a.pre_blocks = static_cast<long long>(a.groups) * kv.kv_heads * p.row_tiles * p.pre_splits;
+    a.m = FastDiv(a.heads / kv.kv_heads);
+    a.row_tiles = FastDiv(p.row_tiles); a.own_tiles = FastDiv(p.own_tiles); a.pre_splits = FastDiv(p.pre_splits); a.own_splits = FastDiv(p.own_splits);
+    a.by_size = FastDiv(a.size); a.by_kv_heads = FastDiv(kv.kv_heads); a.by_vecs = FastDiv(kv.head_dim / 4); a.by_heads = FastDiv(a.heads);
+    a.pre_slots = p.pre_splits; a.slots = p.pre_splits + p.own_splits; a.own_rows = p.own_rows; a.own_warps = p.own_warps;
+    const long long pre_tasks = static_cast<long long>(a.groups) * kv.kv_heads * p.row_tiles * p.pre_splits;
+    const long long own_tasks = static_cast<long long>(a.groups) * a.size * kv.kv_heads * p.own_tiles * p.own_splits;
+    NNB_ARG_CHECK(pre_tasks + own_tasks <= INT_MAX, "too many queries for one call");
+    a.pre_blocks = static_cast<int>(pre_tasks);
+    a.tasks = static_cast<int>(pre_tasks + own_tasks);
+    const long long blocks = pre_tasks + ceil_div(own_tasks, 4 / p.own_warps);
     a.c = 1.4426950408889634f / sqrtf(static_cast<float>(kv.head_dim));
     a.pairs = ((reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.ldq % 2 == 0) ? 1 : 0;
     a.stat = static_cast<float2*>(scratch);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + (rows * a.slots() * 8 + 15) / 16 * 16);
-    const long long blocks = a.pre_blocks + static_cast<long long>(a.groups) * a.size * kv.kv_heads * p.own_tiles * p.own_splits;
-    NNB_ARG_CHECK(blocks <= INT_MAX, "too many queries for one call");
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + (rows * a.slots * 8 + 15) / 16 * 16);
     if (blocks > 0) {
         auto go = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
             NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
@@ -632,12 +912,14 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
         };
         auto width = [&](auto dp) {
             constexpr int DP = decltype(dp)::value;
-            static PerDeviceOnce once[3];
+            static PerDeviceOnce once[6];
             if constexpr (sizeof(T) == 4) return go(paged_attn_f32_kernel<DP>, AttnTile32<DP>::SMEM, once[0]);
             else {
-                if (p.rt == 16) return go(paged_attn_bf16_kernel<DP, 1>, AttnTile<DP>::SMEM, once[0]);
-                if (p.rt == 32) return go(paged_attn_bf16_kernel<DP, 2>, AttnTile<DP>::SMEM, once[1]);
-                return go(paged_attn_bf16_kernel<DP, 4>, AttnTile<DP>::SMEM, once[2]);
+                constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::SMEM);
+                const bool wide = p.own_rows == 16;
+                if (p.rt <= 16) return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::SMEM, once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::SMEM, once[1]);
+                if (p.rt == 32) return wide ? go(paged_attn_bf16_kernel<DP, 2, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 2, 1>, both, once[3]);
+                return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[4]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[5]);
             }
         };
         if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
@@ -645,7 +927,7 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
         else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
         else NNB_TRY(width(std::integral_constant<int, 256>()));
     }
-    if (a.slots() == 1) return 0;
+    if (a.slots == 1) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows));
     cfg.blockDim = dim3(128);
