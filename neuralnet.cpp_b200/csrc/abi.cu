@@ -132,6 +132,9 @@ int nnb200_gemm_status(int* host_code)
     int f32g = 0;
     NNB_TRY(f32_gemm_device_error(&f32g));
     if (!*host_code && f32g) *host_code = f32g | 0x08000000;      // bit 27: fp32 GEMM
+    int paged = 0;
+    NNB_TRY(paged_attn_device_error(&paged));
+    if (!*host_code && paged) *host_code = paged | 0x04000000;    // bit 26: attention over a paged cache
     return 0;
 }
 

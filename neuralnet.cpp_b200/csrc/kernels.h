@@ -144,4 +144,7 @@ int attention_fwd_mma(const bf16* qkv, bf16* out, float* lse, const int* doc, in
 int attention_bwd_mma(const bf16* qkv, const bf16* out, const bf16* dout, const float* lse, float* dvec, bf16* dqkv,
                       const int* doc, int B, int S, int H, int dk, int alibi, cudaStream_t s);
 
+// ---- paged_attention.cu : status word of its tcgen05 kernel (reads and clears)
+int paged_attn_device_error(int* code);
+
 }  // namespace nnb

@@ -28,9 +28,10 @@ struct PagedAttnArgs {
     FastDiv pre_splits, own_splits; // blocks that share a prefix, a sequence's own rows (0: divisor 1, and no task)
     FastDiv by_size, by_kv_heads, by_vecs, by_heads;
     int slots, pre_slots, own_rows; // places of a query row's partial results, the prefix's among them; rows of an own tile
-    int own_warps;                  // warps that share a task of own rows: 4, or 1 (four tasks in a block)
+    int own_warps;                  // warps that share a task of own rows: all of a block, or 1 (a task for each)
+    unsigned long long deal;        // tcgen05 kernel: prefix blocks among the blocks before block b are b * deal / 2^32
     int pre_blocks, tasks;          // tasks [0, pre_blocks) are prefixes, a block each; the others own rows
-    int pairs;                      // queries may be read two columns at a time
+    int pairs, vectors;             // queries may be read two columns, or 16 bytes, at a time
     float c;                        // log2(e) / sqrt(head_dim): exponentials are powers of two
     float* part;                    // (query row, slot): head_dim sums
     float2* stat;                   // (query row, slot): maximum (in powers of two) and sum; sum 0: nothing there
@@ -367,7 +368,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
 }
 
 // Up to 16 query rows: nothing is shared between warps, so each warp streams cached rows through a ring of its own, KW rows a
-// step, without a barrier, and the WT warps of a task (one, or the block's four) take its steps in turn and are joined at the
+// step, without a barrier, and the warps of a task (one, or all NW of the block) take its steps in turn and are joined at the
 // end.  The products are transposed, S' = K Q' and O' = V' P', so that cached rows fill the 16 rows of a tensor core tile and
 // queries its 8 columns (NQ = 1 or 2 of them): one query costs half of what it would as one of 16 rows.  P' comes out of the
 // first product with cached rows down and queries across; the second wants it the other way round, an 8 x 8 transposition.
@@ -377,7 +378,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
 template <int DP> struct AttnStream {
     static constexpr int KW = DP <= 32 ? 32 : 16, ST = DP <= 64 ? 3 : 2, PITCH = DP * 2 + 16, CPR = DP / 8;
     static constexpr int PLANE = KW * PITCH, STAGE = 2 * PLANE, RING = ST * STAGE;
-    static constexpr int SMEM = 4 * (RING + 16);
+    static constexpr int smem(int warps) { return warps * (RING + 16); }
 };
 // what a score may be above the reference point of its row's exponentials, in powers of two: sums stay far from overflow
 constexpr float kAttnSlack = 8.0f;
@@ -389,7 +390,7 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t v)
     return r;
 }
 
-template <int DP, int NQ>
+template <int DP, int NQ, int NW>
 __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const PagedAttnArgs& a, const AttnTask& k, uint8_t* smem, int wt)
 {
     using Str = AttnStream<DP>;
@@ -397,7 +398,7 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wk = wt == 1 ? 0 : warp, dk = pool.dk;
     const int all = (k.end - k.begin + KW - 1) / KW, steps = (all - wk + wt - 1) / wt;
     const uint32_t ring = smem_u32(smem) + warp * Str::RING;
-    uint32_t* alive = reinterpret_cast<uint32_t*>(smem + 4 * Str::RING) + warp * 4;
+    uint32_t* alive = reinterpret_cast<uint32_t*>(smem + NW * Str::RING) + warp * 4;
     // the cached row this lane looks up for a step (lanes beyond KW: none)
     auto look = [&](int step) {
         const int t = k.begin + (step * wt + wk) * KW + lane;
@@ -604,12 +605,12 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
             top = sml[r].x; sum = sml[r].y;
         } else {
             const float* s0 = reinterpret_cast<const float*>(smem);
-            float2 st[4];
+            float2 st[NW];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) { st[w] = *reinterpret_cast<const float2*>(s0 + w * (Str::RING / 4) + NQ * 8 * LD + 2 * r); top = fmaxf(top, st[w].x); }
+            for (int w = 0; w < NW; ++w) { st[w] = *reinterpret_cast<const float2*>(s0 + w * (Str::RING / 4) + NQ * 8 * LD + 2 * r); top = fmaxf(top, st[w].x); }
             const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float e = exp2_fast(st[w].x - ref);
                 const float4 y = *reinterpret_cast<const float4*>(s0 + w * (Str::RING / 4) + r * LD + c);
                 sum = fmaf(st[w].y, e, sum);
@@ -620,25 +621,323 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
     }
 }
 
+// own rows, tasks counted from a.pre_blocks: block b of them takes one with all its warps, or one with each
+template <int DP, int NQ, int NW, int RT>
+__device__ __forceinline__ void own_bf16(const PagedPool<bf16>& pool, const PagedAttnArgs& a, int b, uint8_t* smem)
+{
+    const bool shared = a.own_warps != 1;
+    const int task = a.pre_blocks + (shared ? b : b * NW + static_cast<int>(threadIdx.x >> 5));
+    if (task >= a.tasks) return;
+    const AttnTask k = task_of<RT>(pool, a, task);
+    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, shared ? threadIdx.x : threadIdx.x & 31, shared ? 32 * NW : 32); return; }
+    stream_bf16<DP, NQ, NW>(pool, a, k, smem, a.own_warps);
+}
+
 template <int DP, int WM, int NQ>
 __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a)
 {
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int RT = WM == 1 ? NQ * 8 : WM * 16;
     const int b = static_cast<int>(blockIdx.x);
-    if (b < a.pre_blocks) {
-        const AttnTask k = task_of<WM == 1 ? NQ * 8 : WM * 16>(pool, a, b);
-        if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 128); return; }
-        if constexpr (WM == 1) stream_bf16<DP, NQ>(pool, a, k, smem, 4);
-        else attend_bf16<DP, WM>(pool, a, k, smem);
-        return;
+    if (b >= a.pre_blocks) { own_bf16<DP, NQ, 4, RT>(pool, a, b - a.pre_blocks, smem); return; }
+    const AttnTask k = task_of<RT>(pool, a, b);
+    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 128); return; }
+    if constexpr (WM == 1) stream_bf16<DP, NQ, 4>(pool, a, k, smem, 4);
+    else attend_bf16<DP, WM>(pool, a, k, smem);
+}
+
+// ---------------------------------------------------------------- bf16: tcgen05 tiles
+// More than 16 query rows on the 5th-generation tensor cores: 128 rows (those that are not there are zero) against 64 cached
+// rows a step.  S = Q K' (128 x 64) goes to one of two score buffers in TMEM, O (128 x DP) stays in TMEM across steps.
+//   warp 0     looks up the step's pages and loads their rows by TMA, a box of a page (64 rows of a larger one) per lane; pages
+//              that are not there are loaded from behind the pool's end, where TMA fills in zeros
+//   warp 1     issues the products: S of a step two ahead, then O += P V
+//   warps 2-5  a thread per query row: reads its 64 scores, makes P (bf16, shared memory) with the reference point of the
+//              exponentials moved, and O rescaled, only when a score is more than 2^8 above it; V's rows behind the end are
+//              zeroed by these warps before P is handed over, because a page's unused rows may hold anything
+// Bound by the exponentials (128 x 64 of them at 16 a clock: 512 clocks a step, the products at DP = 128 as much): one chain per
+// block takes about 800, so that two blocks on an SM, or one beside blocks that stream own rows, come near it.
+// Every wait is bounded; one that gives up raises a status word, which the others see, and the block drains.
+__device__ int g_paged_attn_error = 0;
+
+template <int DP> struct AttnTc {
+    static constexpr int NS = DP / 64, ST = DP == 64 ? 3 : 2, KT = 64;
+    static constexpr int Q_SUB = 128 * 128, K_SUB = KT * 128;   // bytes of 128 query rows, or 64 cached ones, by 64 columns
+    static constexpr int K_TILE = NS * K_SUB;
+    static constexpr int OFF_K = NS * Q_SUB, OFF_V = OFF_K + ST * K_TILE, OFF_P = OFF_V + ST * K_TILE, OFF_BAR = OFF_P + Q_SUB, TILES = OFF_BAR + 256;
+    static constexpr int WARPS = 6;
+    static constexpr int SMEM = TILES > AttnStream<DP>::smem(WARPS) ? TILES : AttnStream<DP>::smem(WARPS);
+    static constexpr uint32_t TMEM_COLS = 256;                  // scores [0, 128), O [128, 128 + DP)
+};
+
+template <int DP>
+__device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const PagedAttnArgs& a, const AttnTask& k, const CUtensorMap* tk, const CUtensorMap* tv,
+                                          uint8_t* smem)
+{
+    using Tc = AttnTc<DP>;
+    constexpr int ST = Tc::ST, NS = Tc::NS, KT = Tc::KT;
+    uint8_t *sQ = smem, *sK = smem + Tc::OFF_K, *sV = smem + Tc::OFF_V, *sP = smem + Tc::OFF_P;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tc::OFF_BAR);
+    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST, p_full = s_full + 16,
+                   pv_done = s_full + 24, q_full = s_full + 32;
+    uint64_t* alive = bars + 4 * ST + 5;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(alive + ST);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dk = pool.dk, ps = 1 << pool.page_shift;
+    const int steps = (k.end - k.begin + KT - 1) / KT;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 1); mbar_init(v_empty + 8 * i, 1); }
+        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_full, 4); mbar_init(pv_done, 1); mbar_init(q_full, 4);
+        *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;         // the swizzled tiles need a 1024-byte aligned base
+        if (*abort_flag) atomicCAS(&g_paged_attn_error, 0, 9 << 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    // own rows: a task for the block, or one for each of its warps
-    const int task = a.own_warps == 4 ? b : a.pre_blocks + (b - a.pre_blocks) * 4 + static_cast<int>(threadIdx.x >> 5);
-    if (task >= a.tasks) return;
-    const AttnTask k = task_of<WM == 1 ? NQ * 8 : WM * 16>(pool, a, task);
-    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, a.own_warps == 4 ? threadIdx.x : threadIdx.x & 31, 32 * a.own_warps); return; }
-    stream_bf16<DP, NQ>(pool, a, k, smem, a.own_warps);
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Tc::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot, tmem_o = tmem + 128;
+    constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(KT >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DP >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+    auto wait = [&](uint32_t bar, int parity, int code) -> bool { return mbar_wait(bar, parity & 1, abort_flag, code, &g_paged_attn_error); };
+    auto wait_all = [&](uint32_t bar, int parity, int code) -> bool { return __all_sync(0xffffffffu, wait(bar, parity, code)); };
+
+    if (warp == 0) {
+        const int high = min(ps, KT), boxes = KT / high;        // rows of a box, boxes of a step
+        const int nowhere = pool.pages * pool.kv_heads * ps;    // a row behind the pool
+        bool ok = !*abort_flag;
+        for (int i = 0; ok && i < steps; ++i) {
+            const int st = i % ST, use = i / ST, t = k.begin + i * KT + lane * high;
+            int row = -1;
+            if (lane < boxes && t < k.end) row = pool.find(k.table, k.hk, t);
+            if (!(ok = wait_all(k_empty + 8 * st, use + 1, 1))) break;
+            if (lane == 0) mbar_expect_tx(k_full + 8 * st, Tc::K_TILE);
+            __syncwarp();
+            if (lane < boxes) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j)
+                    tma_load_2d(smem_u32(sK) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tk, k_full + 8 * st, j * 64, row < 0 ? nowhere : row);
+            }
+            // bit r: row r of the step is there
+            const int rows = row < 0 ? 0 : min(high, k.end - t);
+            const unsigned long long mine = rows <= 0 ? 0ull : (rows >= 64 ? ~0ull : (1ull << rows) - 1ull) << (lane < boxes ? lane * high : 0);
+            const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine)), hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine >> 32));
+            if (!(ok = wait_all(v_empty + 8 * st, use + 1, 2))) break;
+            if (lane == 0) {
+                alive[st] = static_cast<uint64_t>(hi) << 32 | lo;
+                mbar_expect_tx(v_full + 8 * st, Tc::K_TILE);
+            }
+            __syncwarp();
+            if (lane < boxes) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j)
+                    tma_load_2d(smem_u32(sV) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tv, v_full + 8 * st, j * 64, row < 0 ? nowhere : row);
+            }
+        }
+        // nothing of this block's is under way when it ends: the last loads are waited for here, whoever gave up
+        if (lane == 0)
+            for (int i = max(0, steps - ST); i < steps; ++i)
+                if (!*abort_flag) { wait(k_full + 8 * (i % ST), i / ST, 3); wait(v_full + 8 * (i % ST), i / ST, 4); }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t q_addr = smem_u32(sQ), p_addr = smem_u32(sP);
+            bool ok = !*abort_flag && wait(q_full, 0, 5);
+            auto issue_s = [&](int i) -> bool {
+                const int st = i % ST;
+                if (!wait(k_full + 8 * st, i / ST, 6)) return false;
+                tc_fence_after();
+                const uint32_t k_addr = smem_u32(sK) + st * Tc::K_TILE;
+#pragma unroll
+                for (int x = 0; x < DP / 16; ++x)
+                    umma_bf16(tmem + (i & 1) * 64, smem_desc(q_addr + (x >> 2) * Tc::Q_SUB + (x & 3) * 32, 16, 1024),
+                              smem_desc(k_addr + (x >> 2) * Tc::K_SUB + (x & 3) * 32, 16, 1024), IDESC_S, x > 0 ? 1u : 0u);
+                umma_commit(s_full + 8 * (i & 1));
+                umma_commit(k_empty + 8 * st);
+                return true;
+            };
+            if (ok) ok = issue_s(0);
+            if (ok && steps > 1) ok = issue_s(1);
+            for (int i = 0; ok && i < steps; ++i) {
+                const int st = i % ST;
+                if (!(ok = wait(p_full, i, 7))) break;          // P is written, the scores of step i are read
+                if (!(ok = wait(v_full + 8 * st, i / ST, 8))) break;
+                tc_fence_after();
+                const uint32_t v_addr = smem_u32(sV) + st * Tc::K_TILE;
+#pragma unroll
+                for (int x = 0; x < KT / 16; ++x)
+                    umma_bf16(tmem_o, smem_desc(p_addr + x * 32, 16, 1024), smem_desc(v_addr + x * 2048, Tc::K_SUB, 1024), IDESC_PV, i > 0 || x > 0 ? 1u : 0u);
+                umma_commit(v_empty + 8 * st);
+                umma_commit(pv_done);
+                if (i + 2 < steps) ok = issue_s(i + 2);
+            }
+        }
+    } else {
+        const int quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+        const int sw = row & 7;
+        const bool live = row < k.rows, work = quad * 32 < k.rows;   // a warp without rows hands over zeros
+        const AttnRow w = row_of(a, k, live ? row : 0);
+        {   // the query row, zero where there is none
+            const bf16* q = static_cast<const bf16*>(a.q) + w.seq * a.ldq + static_cast<long long>(w.head) * dk;
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (live && c * 8 < dk) {
+                    if (a.vectors) v = *reinterpret_cast<const uint4*>(q + c * 8);
+                    else {
+                        alignas(16) bf16 x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = q[c * 8 + e];
+                        v = *reinterpret_cast<const uint4*>(x);
+                    }
+                }
+                *reinterpret_cast<uint4*>(sQ + (c >> 3) * Tc::Q_SUB + row * 128 + (((c & 7) ^ sw) << 4)) = v;
+            }
+        }
+        uint8_t* prow = sP + row * 128;
+        if (!work) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        const float mul = a.alibi ? 1.f : a.c;
+        const float slope = a.alibi && live ? alibi_slope2(w.head, a.heads) : 0.f;
+        const float far = a.alibi && live ? static_cast<float>(far_of(a, pool.page_shift, k, w.seq)) : 0.f;
+        float m = -INFINITY, l = 0.f;
+        bool ok = !*abort_flag;
+        for (int i = 0; ok && i < steps; ++i) {
+            const int st = i % ST;
+            if (!(ok = wait_all(v_full + 8 * st, i / ST, 10))) break;
+            const uint64_t mask = alive[st];
+            if (mask != ~0ull) {
+                for (int idx = threadIdx.x - 64; idx < KT * NS * 8; idx += 128) {
+                    const int r = (idx >> 3) % KT;
+                    if (!(mask >> r & 1ull)) *reinterpret_cast<uint4*>(sV + st * Tc::K_TILE + (idx >> 3) / KT * Tc::K_SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            if (!(ok = wait_all(s_full + 8 * (i & 1), i >> 1, 11))) break;
+            uint32_t p[32];
+            if (work) {
+                tc_fence_after();
+                uint32_t lo[32], hi[32];
+                tmem_ld32(tmem + lanes + (i & 1) * 64, lo);
+                tmem_ld32(tmem + lanes + (i & 1) * 64 + 32, hi);
+                tmem_ld_wait();
+                float x[64];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) { x[j] = __uint_as_float(lo[j]); x[j + 32] = __uint_as_float(hi[j]); }
+                if (a.alibi) {
+                    const float t0 = static_cast<float>(k.begin + i * KT);
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) x[j] = x[j] * a.c - slope * (far - (t0 + static_cast<float>(j)));
+                }
+                if (mask != ~0ull) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) if (!(mask >> j & 1ull)) x[j] = -INFINITY;
+                }
+                float top4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int j = 4; j < 64; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * mul;
+                const bool move = top > m + kAttnSlack;
+                if (__any_sync(0xffffffffu, move)) {
+                    const float back = move ? exp2_fast(m - top) : 1.0f;          // 0 from -inf
+                    if (move) m = top;
+                    l *= back;
+                    if (i > 0) {
+                        if (!(ok = wait_all(pv_done, i - 1, 12))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < DP; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(tmem_o + lanes + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
+                            tmem_st32(tmem_o + lanes + c, o);
+                        }
+                        tmem_st_wait();
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                const uint64_t mul2_ = pack2(mul, mul), ref2 = pack2(-ref, -ref);
+                uint64_t sum2 = 0ull;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float e0, e1;
+                    unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul2_, ref2), e0, e1);
+                    e0 = exp2_fast(e0);
+                    e1 = exp2_fast(e1);
+                    sum2 = add2(sum2, pack2(e0, e1));
+                    p[j] = pack_bf16x2(e0, e1);                 // rounded for the tensor cores, summed as they are
+                }
+                float s0, s1;
+                unpack2(sum2, s0, s1);
+                l += s0 + s1;
+            }
+            if (i > 0 && !(ok = wait_all(pv_done, i - 1, 13))) break;             // P of the step before is used up
+            if (work) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + ((c ^ sw) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+            }
+            tc_fence_before();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full);
+        }
+        if (ok && work && wait_all(pv_done, steps - 1, 14)) {
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(tmem_o + lanes + c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (live && c + j < dk)
+                        leave<bf16>(a, k, dk, row, c + j, make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3])), m, l);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Tc::TMEM_COLS) : "memory");
+    }
+}
+
+// Prefix blocks, bound by the tensor cores and exponentials, and blocks of own rows, bound by memory, are dealt out mixed, the
+// prefix's somewhat ahead, so that an SM holds one of each most of the time.
+template <int DP, int NQ>
+__global__ void __launch_bounds__(192, 2) paged_attn_tc_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap tk,
+                                                               const __grid_constant__ CUtensorMap tv)
+{
+    extern __shared__ __align__(1024) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const unsigned long long b = blockIdx.x;
+    const int p0 = static_cast<int>(min(b * a.deal >> 32, static_cast<unsigned long long>(a.pre_blocks)));
+    const int p1 = static_cast<int>(min((b + 1) * a.deal >> 32, static_cast<unsigned long long>(a.pre_blocks)));
+    if (p1 == p0) { own_bf16<DP, NQ, AttnTc<DP>::WARPS, 128>(pool, a, static_cast<int>(b) - p0, smem); return; }
+    const AttnTask k = task_of<128>(pool, a, p0);
+    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 192); return; }
+    attend_tc<DP>(pool, a, k, &tk, &tv, smem);
+}
+
+int paged_attn_device_error(int* code)
+{
+    NNB_CUDA_CHECK(cudaMemcpyFromSymbol(code, g_paged_attn_error, sizeof(int)));
+    if (*code) { const int z = 0; NNB_CUDA_CHECK(cudaMemcpyToSymbol(g_paged_attn_error, &z, sizeof(int))); }
+    return 0;
 }
 
 // ---------------------------------------------------------------- fp32: FMA tiles
@@ -681,7 +980,7 @@ __device__ __forceinline__ void load_f32(const PagedPool<float>& pool, const Att
 template <int DP>
 __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> pool, const __grid_constant__ PagedAttnArgs a)
 {
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     using Tile = AttnTile32<DP>;
     constexpr int KT = Tile::KT, ST = Tile::STAGES, PL = Tile::PL;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -861,26 +1160,30 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------- how the work is cut
-struct AttnPlan { int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps; };
+struct AttnPlan { bool tc; int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps, block_warps; };
 static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int heads, int prefix_stride, int table_stride)
 {
     AttnPlan p;
     const int m = heads / kv.kv_heads;
     const long long rows = static_cast<long long>(size) * m;
-    // fp32 tiles take 16 query rows; bf16 streams 8 or 16, the shared tiles 32 or 64
-    p.rt = kv.dtype == 0 ? 16 : (rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 64)));
+    // fp32 tiles take 16 query rows; bf16 streams 8 or 16; beyond that tcgen05 tiles take 128, and where a head is too wide
+    // for those mma.sync tiles take 64
+    p.tc = kv.dtype == 1 && rows > 16 && kv.head_dim <= 128 && prefix_stride > 0;
+    p.rt = kv.dtype == 0 ? 16 : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : 64)));
     p.own_rows = kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16)) ? 8 : 16;
     p.row_tiles = static_cast<int>(ceil_div(rows, p.rt));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
+    p.block_warps = p.tc ? 6 : 4;
     const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
     const long long pre_units = static_cast<long long>(groups) * kv.kv_heads * p.row_tiles, own_units = static_cast<long long>(groups) * size * kv.kv_heads * p.own_tiles;
     // cached rows for a block when the tables are full: enough blocks for the machine a few times over, at least two steps each
     const long long blocks = 148LL * 8;
-    long long chunk = ceil_div(pre_units * pre + own_units * own, blocks);
+    long long chunk = ceil_div((p.tc ? 0 : pre_units * pre) + own_units * own, blocks);
     chunk = std::min<long long>(std::max<long long>(ceil_div(chunk, 64) * 64, 128), 1 << 20);
     p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
+    if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / pre_units, 1), ceil_div(pre, 512)));
     p.own_splits = static_cast<int>(ceil_div(own, chunk));
-    p.own_warps = kv.dtype == 0 || ceil_div(own, std::max(1, p.own_splits)) > 512 ? 4 : 1;
+    p.own_warps = kv.dtype == 0 || ceil_div(own, std::max(1, p.own_splits)) > 512 ? p.block_warps : 1;
     return p;
 }
 
@@ -898,9 +1201,11 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
     NNB_ARG_CHECK(pre_tasks + own_tasks <= INT_MAX, "too many queries for one call");
     a.pre_blocks = static_cast<int>(pre_tasks);
     a.tasks = static_cast<int>(pre_tasks + own_tasks);
-    const long long blocks = pre_tasks + ceil_div(own_tasks, 4 / p.own_warps);
+    const long long blocks = pre_tasks + ceil_div(own_tasks, p.block_warps / p.own_warps);
+    if (blocks > 0) a.deal = std::min(1ull << 32, ((static_cast<unsigned long long>(pre_tasks) << 32) / 4 * 5 + blocks - 1) / blocks);
     a.c = 1.4426950408889634f / sqrtf(static_cast<float>(kv.head_dim));
     a.pairs = ((reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.ldq % 2 == 0) ? 1 : 0;
+    a.vectors = ((reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0) ? 1 : 0;
     a.stat = static_cast<float2*>(scratch);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + (rows * a.slots * 8 + 15) / 16 * 16);
     if (blocks > 0) {
@@ -912,17 +1217,35 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
         };
         auto width = [&](auto dp) {
             constexpr int DP = decltype(dp)::value;
-            static PerDeviceOnce once[6];
+            static PerDeviceOnce once[4];
             if constexpr (sizeof(T) == 4) return go(paged_attn_f32_kernel<DP>, AttnTile32<DP>::SMEM, once[0]);
             else {
-                constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::SMEM);
                 const bool wide = p.own_rows == 16;
-                if (p.rt <= 16) return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::SMEM, once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::SMEM, once[1]);
-                if (p.rt == 32) return wide ? go(paged_attn_bf16_kernel<DP, 2, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 2, 1>, both, once[3]);
-                return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[4]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[5]);
+                if constexpr (DP == 256) {
+                    constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));
+                    if (p.rt == 64) return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[3]);
+                }
+                return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::smem(4), once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::smem(4), once[1]);
             }
         };
-        if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
+        if constexpr (sizeof(T) == 2) if (p.tc) {
+            const long long pool_rows = static_cast<long long>(kv.pages) * kv.kv_heads * kv.page_size;
+            CUtensorMap tk, tv;
+            NNB_TRY(tensor_map_2d(pool.k, kv.head_dim, pool_rows, kv.head_dim, 64, std::min(kv.page_size, 64), &tk, 2));
+            NNB_TRY(tensor_map_2d(pool.v, kv.head_dim, pool_rows, kv.head_dim, 64, std::min(kv.page_size, 64), &tv, 2));
+            auto tc = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
+                NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
+                kernel<<<static_cast<unsigned>(blocks), 192, bytes, s>>>(pool, a, tk, tv);
+                NNB_LAUNCH_CHECK();
+                return 0;
+            };
+            static PerDeviceOnce once[4];
+            const bool wide = p.own_rows == 16;
+            if (kv.head_dim <= 64) NNB_TRY(wide ? tc(paged_attn_tc_kernel<64, 2>, AttnTc<64>::SMEM, once[0]) : tc(paged_attn_tc_kernel<64, 1>, AttnTc<64>::SMEM, once[1]));
+            else NNB_TRY(wide ? tc(paged_attn_tc_kernel<128, 2>, AttnTc<128>::SMEM, once[2]) : tc(paged_attn_tc_kernel<128, 1>, AttnTc<128>::SMEM, once[3]));
+        }
+        if (p.tc) {}
+        else if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
         else if (kv.head_dim <= 64) NNB_TRY(width(std::integral_constant<int, 64>()));
         else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
         else NNB_TRY(width(std::integral_constant<int, 256>()));
