@@ -29,7 +29,6 @@ struct PagedAttnArgs {
     FastDiv by_size, by_kv_heads, by_vecs, by_heads;
     int slots, pre_slots, own_rows; // places of a query row's partial results, the prefix's among them; rows of an own tile
     int own_warps;                  // warps that share a task of own rows: all of a block, or 1 (a task for each)
-    unsigned long long deal;        // tcgen05 kernel: prefix blocks among the blocks before block b are b * deal / 2^32
     int pre_blocks, tasks;          // tasks [0, pre_blocks) are prefixes, a block each; the others own rows
     int pairs, vectors;             // queries may be read two columns, or 16 bytes, at a time
     float c;                        // log2(e) / sqrt(head_dim): exponentials are powers of two
@@ -414,7 +413,7 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
     auto fetch = [&](int row, int stage) {
         const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
         if (lane == 0) alive[stage] = mask;
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < KW / RPI; ++i) {
             const int r = __shfl_sync(0xffffffffu, row, i * RPI + lane / CPR);
             const long long off = static_cast<long long>(max(r, 0)) * (dk * 2);
@@ -576,7 +575,7 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
             for (int w = 4; w < 32; w <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], w);
     cp_wait<0>();
     if (wt == 1) __syncwarp();
-    else __syncthreads();
+    else asm volatile("barrier.cta.sync 0, %0;" ::"n"(32 * NW) : "memory");
     // through shared memory, so that rows are written with whole vectors; the warps of a task are joined on the way
     constexpr int LD = DP + 4;
     static_assert(NQ * 8 * (LD * 4 + 8) <= Str::RING, "the join fits a warp's ring");
@@ -594,7 +593,7 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
             }
         }
     if (wt == 1) __syncwarp();
-    else __syncthreads();
+    else asm volatile("barrier.cta.sync 0, %0;" ::"n"(32 * NW) : "memory");
     const int vecs = dk / 4;
     for (int idx = wt == 1 ? lane : threadIdx.x; idx < k.rows * vecs; idx += 32 * wt) {
         const int r = a.by_vecs.div(idx), c = (idx - r * vecs) * 4;
@@ -653,23 +652,38 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
 //   warp 0     looks up the step's pages and loads their rows by TMA, a box of a page (64 rows of a larger one) per lane; pages
 //              that are not there are loaded from behind the pool's end, where TMA fills in zeros
 //   warp 1     issues the products: S of a step two ahead, then O += P V
-//   warps 2-5  a thread per query row: reads its 64 scores, makes P (bf16, shared memory) with the reference point of the
-//              exponentials moved, and O rescaled, only when a score is more than 2^8 above it; V's rows behind the end are
-//              zeroed by these warps before P is handed over, because a page's unused rows may hold anything
-// Bound by the exponentials (128 x 64 of them at 16 a clock: 512 clocks a step, the products at DP = 128 as much): one chain per
-// block takes about 800, so that two blocks on an SM, or one beside blocks that stream own rows, come near it.
-// Every wait is bounded; one that gives up raises a status word, which the others see, and the block drains.
+//   warps 2-9  two threads per query row, half of the columns each: read their 32 scores, make P (bf16, shared memory) with the
+//              reference point of the exponentials moved, and O rescaled, only when a score is more than 2^8 above it (the one
+//              thing the two must agree on); V's rows behind the end are zeroed by these warps before P is handed over,
+//              because a page's unused rows may hold anything
+// A step is a chain of waits, reads, exponentials (64 rows' worth of 8 clocks a warp) and hand-overs; two blocks an SM overlap two.
+// Every wait is bounded; one that gives up raises a status word, the others see it, and the block drains: the two threads of a
+// row leave together, at the barrier where they compare notes.
 __device__ int g_paged_attn_error = 0;
 
 template <int DP> struct AttnTc {
     static constexpr int NS = DP / 64, ST = DP == 64 ? 3 : 2, KT = 64;
     static constexpr int Q_SUB = 128 * 128, K_SUB = KT * 128;   // bytes of 128 query rows, or 64 cached ones, by 64 columns
     static constexpr int K_TILE = NS * K_SUB;
-    static constexpr int OFF_K = NS * Q_SUB, OFF_V = OFF_K + ST * K_TILE, OFF_P = OFF_V + ST * K_TILE, OFF_BAR = OFF_P + Q_SUB, TILES = OFF_BAR + 256;
-    static constexpr int WARPS = 6;
-    static constexpr int SMEM = TILES > AttnStream<DP>::smem(WARPS) ? TILES : AttnStream<DP>::smem(WARPS);
+    static constexpr int OFF_K = NS * Q_SUB, OFF_V = OFF_K + ST * K_TILE, OFF_P = OFF_V + ST * K_TILE, OFF_X = OFF_P + Q_SUB, OFF_BAR = OFF_X + 2 * 128 * 2;
+    static constexpr int TILES = OFF_BAR + 256;                 // DP = 128: two blocks fit an SM, with 256 bytes to spare
+    static constexpr int WARPS = 10, OWN_WARPS = DP == 64 ? 8 : 6;   // warps, and those that stream own rows
+    static constexpr int SMEM = TILES > AttnStream<DP>::smem(OWN_WARPS) ? TILES : AttnStream<DP>::smem(OWN_WARPS);
     static constexpr uint32_t TMEM_COLS = 256;                  // scores [0, 128), O [128, 128 + DP)
 };
+
+// barrier of the two warps that share 32 query rows, and the OR of a flag over them
+__device__ __forceinline__ bool pair_any(int quad, bool pred)
+{
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "barrier.cta.red.or.pred p, %1, 64, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r) : "r"(quad + 1), "r"(static_cast<uint32_t>(pred)) : "memory");
+    return r != 0;
+}
 
 template <int DP>
 __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const PagedAttnArgs& a, const AttnTask& k, const CUtensorMap* tk, const CUtensorMap* tv,
@@ -678,19 +692,21 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     using Tc = AttnTc<DP>;
     constexpr int ST = Tc::ST, NS = Tc::NS, KT = Tc::KT;
     uint8_t *sQ = smem, *sK = smem + Tc::OFF_K, *sV = smem + Tc::OFF_V, *sP = smem + Tc::OFF_P;
+    bf16* sX = reinterpret_cast<bf16*>(smem + Tc::OFF_X);       // (half, row)
+    float* sL = reinterpret_cast<float*>(sQ);                   // (half, row), once the query tile has been used
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tc::OFF_BAR);
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST, p_full = s_full + 16,
                    pv_done = s_full + 24, q_full = s_full + 32;
-    uint64_t* alive = bars + 4 * ST + 5;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(alive + ST);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * ST + 5);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dk = pool.dk, ps = 1 << pool.page_shift;
     const int steps = (k.end - k.begin + KT - 1) / KT;
+    const int high = min(ps, KT), boxes = KT / high;            // rows of a box, boxes of a step
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 1); mbar_init(v_empty + 8 * i, 1); }
-        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_full, 4); mbar_init(pv_done, 1); mbar_init(q_full, 4);
+        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_full, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8);
         *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;         // the swizzled tiles need a 1024-byte aligned base
         if (*abort_flag) atomicCAS(&g_paged_attn_error, 0, 9 << 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -708,37 +724,32 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DP >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     auto wait = [&](uint32_t bar, int parity, int code) -> bool { return mbar_wait(bar, parity & 1, abort_flag, code, &g_paged_attn_error); };
     auto wait_all = [&](uint32_t bar, int parity, int code) -> bool { return __all_sync(0xffffffffu, wait(bar, parity, code)); };
+    // first row in the pool of the box this lane has of step i, -1: it is not there (the whole warp calls this)
+    auto box_of = [&](int i) -> int {
+        const int t = k.begin + i * KT + lane * high;
+        return i < steps && lane < boxes && t < k.end ? pool.find(k.table, k.hk, t) : -1;
+    };
 
     if (warp == 0) {
-        const int high = min(ps, KT), boxes = KT / high;        // rows of a box, boxes of a step
         const int nowhere = pool.pages * pool.kv_heads * ps;    // a row behind the pool
         bool ok = !*abort_flag;
+        int row = box_of(0);
         for (int i = 0; ok && i < steps; ++i) {
-            const int st = i % ST, use = i / ST, t = k.begin + i * KT + lane * high;
-            int row = -1;
-            if (lane < boxes && t < k.end) row = pool.find(k.table, k.hk, t);
+            const int st = i % ST, use = i / ST, y = row < 0 ? nowhere : row;
             if (!(ok = wait_all(k_empty + 8 * st, use + 1, 1))) break;
             if (lane == 0) mbar_expect_tx(k_full + 8 * st, Tc::K_TILE);
             __syncwarp();
             if (lane < boxes) {
 #pragma unroll
-                for (int j = 0; j < NS; ++j)
-                    tma_load_2d(smem_u32(sK) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tk, k_full + 8 * st, j * 64, row < 0 ? nowhere : row);
+                for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sK) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tk, k_full + 8 * st, j * 64, y);
             }
-            // bit r: row r of the step is there
-            const int rows = row < 0 ? 0 : min(high, k.end - t);
-            const unsigned long long mine = rows <= 0 ? 0ull : (rows >= 64 ? ~0ull : (1ull << rows) - 1ull) << (lane < boxes ? lane * high : 0);
-            const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine)), hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine >> 32));
+            row = box_of(i + 1);
             if (!(ok = wait_all(v_empty + 8 * st, use + 1, 2))) break;
-            if (lane == 0) {
-                alive[st] = static_cast<uint64_t>(hi) << 32 | lo;
-                mbar_expect_tx(v_full + 8 * st, Tc::K_TILE);
-            }
+            if (lane == 0) mbar_expect_tx(v_full + 8 * st, Tc::K_TILE);
             __syncwarp();
             if (lane < boxes) {
 #pragma unroll
-                for (int j = 0; j < NS; ++j)
-                    tma_load_2d(smem_u32(sV) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tv, v_full + 8 * st, j * 64, row < 0 ? nowhere : row);
+                for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sV) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tv, v_full + 8 * st, j * 64, y);
             }
         }
         // nothing of this block's is under way when it ends: the last loads are waited for here, whoever gave up
@@ -747,17 +758,17 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                 if (!*abort_flag) { wait(k_full + 8 * (i % ST), i / ST, 3); wait(v_full + 8 * (i % ST), i / ST, 4); }
     } else if (warp == 1) {
         if (lane == 0) {
-            const uint32_t q_addr = smem_u32(sQ), p_addr = smem_u32(sP);
             bool ok = !*abort_flag && wait(q_full, 0, 5);
+            const uint64_t dq = smem_desc(smem_u32(sQ), 16, 1024), dkey = smem_desc(smem_u32(sK), 16, 1024), dp = smem_desc(smem_u32(sP), 16, 1024),
+                           dv = smem_desc(smem_u32(sV), Tc::K_SUB, 1024);        // addresses in units of 16 bytes: offsets are added below
             auto issue_s = [&](int i) -> bool {
                 const int st = i % ST;
                 if (!wait(k_full + 8 * st, i / ST, 6)) return false;
                 tc_fence_after();
-                const uint32_t k_addr = smem_u32(sK) + st * Tc::K_TILE;
 #pragma unroll
                 for (int x = 0; x < DP / 16; ++x)
-                    umma_bf16(tmem + (i & 1) * 64, smem_desc(q_addr + (x >> 2) * Tc::Q_SUB + (x & 3) * 32, 16, 1024),
-                              smem_desc(k_addr + (x >> 2) * Tc::K_SUB + (x & 3) * 32, 16, 1024), IDESC_S, x > 0 ? 1u : 0u);
+                    umma_bf16(tmem + (i & 1) * 64, dq + (((x >> 2) * Tc::Q_SUB + (x & 3) * 32) >> 4), dkey + ((st * Tc::K_TILE + (x >> 2) * Tc::K_SUB + (x & 3) * 32) >> 4),
+                              IDESC_S, x > 0 ? 1u : 0u);
                 umma_commit(s_full + 8 * (i & 1));
                 umma_commit(k_empty + 8 * st);
                 return true;
@@ -766,45 +777,44 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
             if (ok && steps > 1) ok = issue_s(1);
             for (int i = 0; ok && i < steps; ++i) {
                 const int st = i % ST;
-                if (!(ok = wait(p_full, i, 7))) break;          // P is written, the scores of step i are read
                 if (!(ok = wait(v_full + 8 * st, i / ST, 8))) break;
+                if (!(ok = wait(p_full, i, 7))) break;          // P is written, the scores of step i are read
                 tc_fence_after();
-                const uint32_t v_addr = smem_u32(sV) + st * Tc::K_TILE;
 #pragma unroll
-                for (int x = 0; x < KT / 16; ++x)
-                    umma_bf16(tmem_o, smem_desc(p_addr + x * 32, 16, 1024), smem_desc(v_addr + x * 2048, Tc::K_SUB, 1024), IDESC_PV, i > 0 || x > 0 ? 1u : 0u);
-                umma_commit(v_empty + 8 * st);
+                for (int x = 0; x < KT / 16; ++x) umma_bf16(tmem_o, dp + (x * 32 >> 4), dv + ((st * Tc::K_TILE + x * 2048) >> 4), IDESC_PV, i > 0 || x > 0 ? 1u : 0u);
                 umma_commit(pv_done);
+                umma_commit(v_empty + 8 * st);
                 if (i + 2 < steps) ok = issue_s(i + 2);
             }
         }
     } else {
-        const int quad = warp & 3, row = quad * 32 + lane;
+        const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const int sw = row & 7;
-        const bool live = row < k.rows, work = quad * 32 < k.rows;   // a warp without rows hands over zeros
+        const bool live = row < k.rows, work = quad * 32 < k.rows;   // warps without rows hand over zeros
         const AttnRow w = row_of(a, k, live ? row : 0);
-        {   // the query row, zero where there is none
+        {   // half of the query row, zero where there is none
             const bf16* q = static_cast<const bf16*>(a.q) + w.seq * a.ldq + static_cast<long long>(w.head) * dk;
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
+#pragma unroll 2
+            for (int c = 0; c < DP / 16; ++c) {
+                const int cc = half * (DP / 16) + c;
                 uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (live && c * 8 < dk) {
-                    if (a.vectors) v = *reinterpret_cast<const uint4*>(q + c * 8);
+                if (live && cc * 8 < dk) {
+                    if (a.vectors) v = *reinterpret_cast<const uint4*>(q + cc * 8);
                     else {
                         alignas(16) bf16 x[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = q[c * 8 + e];
+                        for (int e = 0; e < 8; ++e) x[e] = q[cc * 8 + e];
                         v = *reinterpret_cast<const uint4*>(x);
                     }
                 }
-                *reinterpret_cast<uint4*>(sQ + (c >> 3) * Tc::Q_SUB + row * 128 + (((c & 7) ^ sw) << 4)) = v;
+                *reinterpret_cast<uint4*>(sQ + (cc >> 3) * Tc::Q_SUB + row * 128 + (((cc & 7) ^ sw) << 4)) = v;
             }
         }
         uint8_t* prow = sP + row * 128;
         if (!work) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(prow + (half * 4 + c) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -813,98 +823,118 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
         const float slope = a.alibi && live ? alibi_slope2(w.head, a.heads) : 0.f;
         const float far = a.alibi && live ? static_cast<float>(far_of(a, pool.page_shift, k, w.seq)) : 0.f;
         float m = -INFINITY, l = 0.f;
-        bool ok = !*abort_flag;
-        for (int i = 0; ok && i < steps; ++i) {
+        bool bad = *abort_flag != 0;                            // a wait of this thread gave up
+        int box = box_of(0);
+        for (int i = 0; i < steps; ++i) {
             const int st = i % ST;
-            if (!(ok = wait_all(v_full + 8 * st, i / ST, 10))) break;
-            const uint64_t mask = alive[st];
-            if (mask != ~0ull) {
-                for (int idx = threadIdx.x - 64; idx < KT * NS * 8; idx += 128) {
+            // bit r of (lo, hi): row r of the step is there; 64 of them but for the last step and steps with missing pages
+            const int count = box < 0 ? 0 : min(high, k.end - (k.begin + i * KT + lane * high));
+            const bool whole = __all_sync(0xffffffffu, lane >= boxes || count == high);
+            uint32_t lo = 0xffffffffu, hi = 0xffffffffu;
+            if (!whole) {
+                const unsigned long long mine = lane < boxes && count > 0 ? (count >= 64 ? ~0ull : (1ull << count) - 1ull) << (lane * high) : 0ull;
+                lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine));
+                hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine >> 32));
+                bad |= !wait_all(v_full + 8 * st, i / ST, 10);
+                for (int idx = threadIdx.x - 64; idx < KT * NS * 8; idx += 256) {
                     const int r = (idx >> 3) % KT;
-                    if (!(mask >> r & 1ull)) *reinterpret_cast<uint4*>(sV + st * Tc::K_TILE + (idx >> 3) / KT * Tc::K_SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    if (!((r < 32 ? lo : hi) >> (r & 31) & 1u))
+                        *reinterpret_cast<uint4*>(sV + st * Tc::K_TILE + (idx >> 3) / KT * Tc::K_SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
-            if (!(ok = wait_all(s_full + 8 * (i & 1), i >> 1, 11))) break;
-            uint32_t p[32];
+            box = box_of(i + 1);
+            bad |= !wait_all(s_full + 8 * (i & 1), i >> 1, 11);
+            uint32_t p[16];
             if (work) {
                 tc_fence_after();
-                uint32_t lo[32], hi[32];
-                tmem_ld32(tmem + lanes + (i & 1) * 64, lo);
-                tmem_ld32(tmem + lanes + (i & 1) * 64 + 32, hi);
+                uint32_t r[32];
+                tmem_ld32(tmem + lanes + (i & 1) * 64 + half * 32, r);
                 tmem_ld_wait();
-                float x[64];
+                float x[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) { x[j] = __uint_as_float(lo[j]); x[j + 32] = __uint_as_float(hi[j]); }
+                for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(r[j]);
                 if (a.alibi) {
-                    const float t0 = static_cast<float>(k.begin + i * KT);
+                    const float t0 = static_cast<float>(k.begin + i * KT + half * 32);
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) x[j] = x[j] * a.c - slope * (far - (t0 + static_cast<float>(j)));
+                    for (int j = 0; j < 32; ++j) x[j] = x[j] * a.c - slope * (far - (t0 + static_cast<float>(j)));
                 }
-                if (mask != ~0ull) {
+                if (!whole) {
+                    const uint32_t mask = half ? hi : lo;
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) if (!(mask >> j & 1ull)) x[j] = -INFINITY;
+                    for (int j = 0; j < 32; ++j) if (!(mask >> j & 1u)) x[j] = -INFINITY;
                 }
                 float top4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int j = 4; j < 64; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * mul;
-                const bool move = top > m + kAttnSlack;
-                if (__any_sync(0xffffffffu, move)) {
+                for (int j = 4; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
+                float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * mul;
+                if (pair_any(quad, top > m + kAttnSlack || bad)) {
+                    // rounded up: any point at or just above the maximum will do, and both threads take the same
+                    const bf16 mine = __float2bfloat16_ru(top);
+                    sX[half * 128 + row] = mine;
+                    if (pair_any(quad, bad)) { bad = true; break; }              // both warps leave here
+                    top = fmaxf(__bfloat162float(mine), __bfloat162float(sX[(half ^ 1) * 128 + row]));
+                    const bool move = top > m + kAttnSlack;
                     const float back = move ? exp2_fast(m - top) : 1.0f;          // 0 from -inf
                     if (move) m = top;
                     l *= back;
                     if (i > 0) {
-                        if (!(ok = wait_all(pv_done, i - 1, 12))) break;
+                        bad |= !wait_all(pv_done, i - 1, 12);
                         tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < DP; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(tmem_o + lanes + c, o);
+#pragma unroll 1
+                        for (int c = 0; c < DP / 2; c += 32) {
+                            tmem_ld32(tmem_o + lanes + half * (DP / 2) + c, r);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
-                            tmem_st32(tmem_o + lanes + c, o);
+                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * back);
+                            tmem_st32(tmem_o + lanes + half * (DP / 2) + c, r);
                         }
                         tmem_st_wait();
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                const uint64_t mul2_ = pack2(mul, mul), ref2 = pack2(-ref, -ref);
-                uint64_t sum2 = 0ull;
+                const uint64_t mul_2 = pack2(mul, mul), ref_2 = pack2(-ref, -ref);
+                uint64_t sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
+                for (int j = 0; j < 16; ++j) {
                     float e0, e1;
-                    unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul2_, ref2), e0, e1);
+                    unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul_2, ref_2), e0, e1);
                     e0 = exp2_fast(e0);
                     e1 = exp2_fast(e1);
-                    sum2 = add2(sum2, pack2(e0, e1));
+                    if (j & 1) sum1 = add2(sum1, pack2(e0, e1));
+                    else sum0 = add2(sum0, pack2(e0, e1));
                     p[j] = pack_bf16x2(e0, e1);                 // rounded for the tensor cores, summed as they are
                 }
                 float s0, s1;
-                unpack2(sum2, s0, s1);
+                unpack2(add2(sum0, sum1), s0, s1);
                 l += s0 + s1;
             }
-            if (i > 0 && !(ok = wait_all(pv_done, i - 1, 13))) break;             // P of the step before is used up
+            if (i > 0) bad |= !wait_all(pv_done, i - 1, 13);    // P of the step before is used up
             if (work) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + ((c ^ sw) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
-            }
+                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(prow + (((half * 4 + c) ^ sw) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+            } else if (bad) break;
             tc_fence_before();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full);
         }
-        if (ok && work && wait_all(pv_done, steps - 1, 14)) {
-            tc_fence_after();
+        if (work) {
+            bad |= !wait_all(pv_done, steps - 1, 14);
+            sL[half * 128 + row] = l;
+            if (!pair_any(quad, bad)) {
+                l += sL[(half ^ 1) * 128 + row];
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < DP / 2; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_o + lanes + half * (DP / 2) + c, o);
+                    tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(tmem_o + lanes + c, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (live && c + j < dk)
-                        leave<bf16>(a, k, dk, row, c + j, make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3])), m, l);
+                    for (int j = 0; j < 32; j += 4)
+                        if (live && half * (DP / 2) + c + j < dk)
+                            leave<bf16>(a, k, dk, row, half * (DP / 2) + c + j,
+                                        make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3])), m, l);
+                }
             }
         }
     }
@@ -916,20 +946,20 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     }
 }
 
-// Prefix blocks, bound by the tensor cores and exponentials, and blocks of own rows, bound by memory, are dealt out mixed, the
-// prefix's somewhat ahead, so that an SM holds one of each most of the time.
-template <int DP, int NQ>
-__global__ void __launch_bounds__(192, 2) paged_attn_tc_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap tk,
+// Prefix blocks, bound by the tensor cores and exponentials, first; blocks of own rows, bound by memory, as they end.
+template <int DP>
+__global__ void __launch_bounds__(320, 2) paged_attn_tc_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap tk,
                                                                const __grid_constant__ CUtensorMap tv)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const unsigned long long b = blockIdx.x;
-    const int p0 = static_cast<int>(min(b * a.deal >> 32, static_cast<unsigned long long>(a.pre_blocks)));
-    const int p1 = static_cast<int>(min((b + 1) * a.deal >> 32, static_cast<unsigned long long>(a.pre_blocks)));
-    if (p1 == p0) { own_bf16<DP, NQ, AttnTc<DP>::WARPS, 128>(pool, a, static_cast<int>(b) - p0, smem); return; }
-    const AttnTask k = task_of<128>(pool, a, p0);
-    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 192); return; }
+    const int b = static_cast<int>(blockIdx.x);
+    if (b >= a.pre_blocks) {
+        if (threadIdx.x < AttnTc<DP>::OWN_WARPS * 32) own_bf16<DP, 1, AttnTc<DP>::OWN_WARPS, 128>(pool, a, b - a.pre_blocks, smem);
+        return;
+    }
+    const AttnTask k = task_of<128>(pool, a, b);
+    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 320); return; }
     attend_tc<DP>(pool, a, k, &tk, &tv, smem);
 }
 
@@ -1170,10 +1200,10 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     // for those mma.sync tiles take 64
     p.tc = kv.dtype == 1 && rows > 16 && kv.head_dim <= 128 && prefix_stride > 0;
     p.rt = kv.dtype == 0 ? 16 : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : 64)));
-    p.own_rows = kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16)) ? 8 : 16;
+    p.own_rows = p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
     p.row_tiles = static_cast<int>(ceil_div(rows, p.rt));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
-    p.block_warps = p.tc ? 6 : 4;
+    p.block_warps = !p.tc ? 4 : (kv.head_dim <= 64 ? AttnTc<64>::OWN_WARPS : AttnTc<128>::OWN_WARPS);
     const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
     const long long pre_units = static_cast<long long>(groups) * kv.kv_heads * p.row_tiles, own_units = static_cast<long long>(groups) * size * kv.kv_heads * p.own_tiles;
     // cached rows for a block when the tables are full: enough blocks for the machine a few times over, at least two steps each
@@ -1202,7 +1232,6 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
     a.pre_blocks = static_cast<int>(pre_tasks);
     a.tasks = static_cast<int>(pre_tasks + own_tasks);
     const long long blocks = pre_tasks + ceil_div(own_tasks, p.block_warps / p.own_warps);
-    if (blocks > 0) a.deal = std::min(1ull << 32, ((static_cast<unsigned long long>(pre_tasks) << 32) / 4 * 5 + blocks - 1) / blocks);
     a.c = 1.4426950408889634f / sqrtf(static_cast<float>(kv.head_dim));
     a.pairs = ((reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.ldq % 2 == 0) ? 1 : 0;
     a.vectors = ((reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0) ? 1 : 0;
@@ -1235,14 +1264,13 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
             NNB_TRY(tensor_map_2d(pool.v, kv.head_dim, pool_rows, kv.head_dim, 64, std::min(kv.page_size, 64), &tv, 2));
             auto tc = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
                 NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
-                kernel<<<static_cast<unsigned>(blocks), 192, bytes, s>>>(pool, a, tk, tv);
+                kernel<<<static_cast<unsigned>(blocks), 320, bytes, s>>>(pool, a, tk, tv);
                 NNB_LAUNCH_CHECK();
                 return 0;
             };
-            static PerDeviceOnce once[4];
-            const bool wide = p.own_rows == 16;
-            if (kv.head_dim <= 64) NNB_TRY(wide ? tc(paged_attn_tc_kernel<64, 2>, AttnTc<64>::SMEM, once[0]) : tc(paged_attn_tc_kernel<64, 1>, AttnTc<64>::SMEM, once[1]));
-            else NNB_TRY(wide ? tc(paged_attn_tc_kernel<128, 2>, AttnTc<128>::SMEM, once[2]) : tc(paged_attn_tc_kernel<128, 1>, AttnTc<128>::SMEM, once[3]));
+            static PerDeviceOnce once[2];
+            if (kv.head_dim <= 64) NNB_TRY(tc(paged_attn_tc_kernel<64>, AttnTc<64>::SMEM, once[0]));
+            else NNB_TRY(tc(paged_attn_tc_kernel<128>, AttnTc<128>::SMEM, once[1]));
         }
         if (p.tc) {}
         else if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
