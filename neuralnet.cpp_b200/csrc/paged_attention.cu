@@ -647,25 +647,27 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
 }
 
 // ---------------------------------------------------------------- bf16: tcgen05 tiles
-// More than 16 query rows on the 5th-generation tensor cores: 128 rows (those that are not there are zero) against 64 cached
-// rows a step.  S = Q K' (128 x 64) goes to one of two score buffers in TMEM, O (128 x DP) stays in TMEM across steps.
+// More than 16 query rows on the 5th-generation tensor cores: 128 rows (those that are not there are zero) against 128 cached
+// rows a step.  S = Q K' (128 x 128) goes to TMEM, O (128 x DP) stays in TMEM across steps.
 //   warp 0     looks up the step's pages and loads their rows by TMA, a box of a page (64 rows of a larger one) per lane; pages
 //              that are not there are loaded from behind the pool's end, where TMA fills in zeros
-//   warp 1     issues the products: S of a step two ahead, then O += P V
-//   warps 2-9  two threads per query row, half of the columns each: read their 32 scores, make P (bf16, shared memory) with the
-//              reference point of the exponentials moved, and O rescaled, only when a score is more than 2^8 above it (the one
-//              thing the two must agree on); V's rows behind the end are zeroed by these warps before P is handed over,
-//              because a page's unused rows may hold anything
-// A step is a chain of waits, reads, exponentials (64 rows' worth of 8 clocks a warp) and hand-overs; two blocks an SM overlap two.
+//   warp 1     issues the products: S, and O += P V in two halves of 64 cached rows
+//   warps 2-9  two threads per query row, half of the columns each: read their 64 scores, make P (bf16, shared memory, 64 cached
+//              rows at a time) with the reference point of the exponentials moved, and O rescaled, only when a score is more
+//              than 2^8 above it (the one thing the two must agree on); V's rows behind the end are zeroed by these warps
+//              before P is handed over, because a page's unused rows may hold anything
+// A step is a chain - S, maximum, exponentials, P, P V - with the next step's S between the two halves; two blocks an SM overlap
+// two chains.  64 cached rows a step instead (an S of 128 x 64 takes the tensor core as long as one of 128 x 128) had the issue
+// of products as its bound: 2400 clocks for 64 rows and block, 12 products of 130 clocks.
 // Every wait is bounded; one that gives up raises a status word, the others see it, and the block drains: the two threads of a
 // row leave together, at the barrier where they compare notes.
 __device__ int g_paged_attn_error = 0;
 
 template <int DP> struct AttnTc {
-    static constexpr int NS = DP / 64, ST = DP == 64 ? 3 : 2, KT = 64;
-    static constexpr int Q_SUB = 128 * 128, K_SUB = KT * 128;   // bytes of 128 query rows, or 64 cached ones, by 64 columns
-    static constexpr int K_TILE = NS * K_SUB;
-    static constexpr int OFF_K = NS * Q_SUB, OFF_V = OFF_K + ST * K_TILE, OFF_P = OFF_V + ST * K_TILE, OFF_X = OFF_P + Q_SUB, OFF_BAR = OFF_X + 2 * 128 * 2;
+    static constexpr int NS = DP / 64, ST = DP == 64 ? 2 : 1, KT = 128;
+    static constexpr int SUB = 128 * 128;                       // bytes of 128 rows by 64 columns
+    static constexpr int TILE = NS * SUB;
+    static constexpr int OFF_K = TILE, OFF_V = OFF_K + ST * TILE, OFF_P = OFF_V + ST * TILE, OFF_X = OFF_P + SUB, OFF_BAR = OFF_X + 2 * 128 * 2;
     static constexpr int TILES = OFF_BAR + 256;                 // DP = 128: two blocks fit an SM, with 256 bytes to spare
     static constexpr int WARPS = 10, OWN_WARPS = DP == 64 ? 8 : 6;   // warps, and those that stream own rows
     static constexpr int SMEM = TILES > AttnStream<DP>::smem(OWN_WARPS) ? TILES : AttnStream<DP>::smem(OWN_WARPS);
@@ -696,17 +698,17 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     float* sL = reinterpret_cast<float*>(sQ);                   // (half, row), once the query tile has been used
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tc::OFF_BAR);
     const uint32_t bar0 = smem_u32(bars);
-    const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST, p_full = s_full + 16,
-                   pv_done = s_full + 24, q_full = s_full + 32;
+    const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST, s_free = s_full + 8,
+                   p_full = s_full + 16, pv_done = s_full + 24, q_full = s_full + 32;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * ST + 5);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dk = pool.dk, ps = 1 << pool.page_shift;
     const int steps = (k.end - k.begin + KT - 1) / KT;
-    const int high = min(ps, KT), boxes = KT / high;            // rows of a box, boxes of a step
+    const int high = min(ps, 64), boxes = KT / high;            // rows of a box, boxes of a step: a run begins at a multiple of 64
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 1); mbar_init(v_empty + 8 * i, 1); }
-        mbar_init(s_full, 1); mbar_init(s_full + 8, 1); mbar_init(p_full, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8);
+        mbar_init(s_full, 1); mbar_init(s_free, 8); mbar_init(p_full, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8);
         *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;         // the swizzled tiles need a 1024-byte aligned base
         if (*abort_flag) atomicCAS(&g_paged_attn_error, 0, 9 << 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -737,19 +739,19 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
         for (int i = 0; ok && i < steps; ++i) {
             const int st = i % ST, use = i / ST, y = row < 0 ? nowhere : row;
             if (!(ok = wait_all(k_empty + 8 * st, use + 1, 1))) break;
-            if (lane == 0) mbar_expect_tx(k_full + 8 * st, Tc::K_TILE);
+            if (lane == 0) mbar_expect_tx(k_full + 8 * st, Tc::TILE);
             __syncwarp();
             if (lane < boxes) {
 #pragma unroll
-                for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sK) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tk, k_full + 8 * st, j * 64, y);
+                for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sK) + st * Tc::TILE + j * Tc::SUB + lane * high * 128, tk, k_full + 8 * st, j * 64, y);
             }
             row = box_of(i + 1);
             if (!(ok = wait_all(v_empty + 8 * st, use + 1, 2))) break;
-            if (lane == 0) mbar_expect_tx(v_full + 8 * st, Tc::K_TILE);
+            if (lane == 0) mbar_expect_tx(v_full + 8 * st, Tc::TILE);
             __syncwarp();
             if (lane < boxes) {
 #pragma unroll
-                for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sV) + st * Tc::K_TILE + j * Tc::K_SUB + lane * high * 128, tv, v_full + 8 * st, j * 64, y);
+                for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sV) + st * Tc::TILE + j * Tc::SUB + lane * high * 128, tv, v_full + 8 * st, j * 64, y);
             }
         }
         // nothing of this block's is under way when it ends: the last loads are waited for here, whoever gave up
@@ -760,31 +762,41 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
         if (lane == 0) {
             bool ok = !*abort_flag && wait(q_full, 0, 5);
             const uint64_t dq = smem_desc(smem_u32(sQ), 16, 1024), dkey = smem_desc(smem_u32(sK), 16, 1024), dp = smem_desc(smem_u32(sP), 16, 1024),
-                           dv = smem_desc(smem_u32(sV), Tc::K_SUB, 1024);        // addresses in units of 16 bytes: offsets are added below
+                           dv = smem_desc(smem_u32(sV), Tc::SUB, 1024);          // addresses in units of 16 bytes: offsets are added below
             auto issue_s = [&](int i) -> bool {
                 const int st = i % ST;
                 if (!wait(k_full + 8 * st, i / ST, 6)) return false;
                 tc_fence_after();
 #pragma unroll
-                for (int x = 0; x < DP / 16; ++x)
-                    umma_bf16(tmem + (i & 1) * 64, dq + (((x >> 2) * Tc::Q_SUB + (x & 3) * 32) >> 4), dkey + ((st * Tc::K_TILE + (x >> 2) * Tc::K_SUB + (x & 3) * 32) >> 4),
-                              IDESC_S, x > 0 ? 1u : 0u);
-                umma_commit(s_full + 8 * (i & 1));
+                for (int x = 0; x < DP / 16; ++x) {
+                    const int o = ((x >> 2) * Tc::SUB + (x & 3) * 32) >> 4;
+                    umma_bf16(tmem, dq + o, dkey + (st * Tc::TILE >> 4) + o, IDESC_S, x > 0 ? 1u : 0u);
+                }
+                umma_commit(s_full);
                 umma_commit(k_empty + 8 * st);
                 return true;
             };
+            auto issue_pv = [&](int i, int part) -> bool {
+                const int st = i % ST;
+                if (!wait(p_full, 2 * i + part, 7)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    umma_bf16(tmem_o, dp + (x * 32 >> 4), dv + (st * Tc::TILE >> 4) + ((part * 4 + x) * 2048 >> 4), IDESC_PV, i > 0 || part > 0 || x > 0 ? 1u : 0u);
+                umma_commit(pv_done);
+                return true;
+            };
             if (ok) ok = issue_s(0);
-            if (ok && steps > 1) ok = issue_s(1);
             for (int i = 0; ok && i < steps; ++i) {
                 const int st = i % ST;
                 if (!(ok = wait(v_full + 8 * st, i / ST, 8))) break;
-                if (!(ok = wait(p_full, i, 7))) break;          // P is written, the scores of step i are read
-                tc_fence_after();
-#pragma unroll
-                for (int x = 0; x < KT / 16; ++x) umma_bf16(tmem_o, dp + (x * 32 >> 4), dv + ((st * Tc::K_TILE + x * 2048) >> 4), IDESC_PV, i > 0 || x > 0 ? 1u : 0u);
-                umma_commit(pv_done);
+                if (!(ok = issue_pv(i, 0))) break;
+                if (i + 1 < steps) {
+                    if (!(ok = wait(s_free, i, 15))) break;     // the scores of step i are read
+                    if (!(ok = issue_s(i + 1))) break;
+                }
+                if (!(ok = issue_pv(i, 1))) break;
                 umma_commit(v_empty + 8 * st);
-                if (i + 2 < steps) ok = issue_s(i + 2);
             }
         }
     } else {
@@ -808,7 +820,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                         v = *reinterpret_cast<const uint4*>(x);
                     }
                 }
-                *reinterpret_cast<uint4*>(sQ + (cc >> 3) * Tc::Q_SUB + row * 128 + (((cc & 7) ^ sw) << 4)) = v;
+                *reinterpret_cast<uint4*>(sQ + (cc >> 3) * Tc::SUB + row * 128 + (((cc & 7) ^ sw) << 4)) = v;
             }
         }
         uint8_t* prow = sP + row * 128;
@@ -827,46 +839,60 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
         int box = box_of(0);
         for (int i = 0; i < steps; ++i) {
             const int st = i % ST;
-            // bit r of (lo, hi): row r of the step is there; 64 of them but for the last step and steps with missing pages
-            const int count = box < 0 ? 0 : min(high, k.end - (k.begin + i * KT + lane * high));
+            // bit r of there[p]: row p * 64 + half * 32 + r of the step is there; all of them but for the last step and missing pages
+            const int t0 = k.begin + i * KT, count = box < 0 ? 0 : min(high, k.end - (t0 + lane * high));
             const bool whole = __all_sync(0xffffffffu, lane >= boxes || count == high);
-            uint32_t lo = 0xffffffffu, hi = 0xffffffffu;
+            uint32_t there[2] = {0xffffffffu, 0xffffffffu};
             if (!whole) {
-                const unsigned long long mine = lane < boxes && count > 0 ? (count >= 64 ? ~0ull : (1ull << count) - 1ull) << (lane * high) : 0ull;
-                lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine));
-                hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine >> 32));
+                // rows [from, from + count) of the step are this lane's, as bits of its 128
+                const int from = lane * high;
+                uint32_t word[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int b0 = max(from - x * 32, 0), b1 = min(from + (lane < boxes ? count : 0) - x * 32, 32);
+                    word[x] = __reduce_or_sync(0xffffffffu, b1 <= b0 ? 0u : (b1 - b0 == 32 ? 0xffffffffu : ((1u << (b1 - b0)) - 1u) << b0));
+                }
+                there[0] = half ? word[1] : word[0];
+                there[1] = half ? word[3] : word[2];
                 bad |= !wait_all(v_full + 8 * st, i / ST, 10);
                 for (int idx = threadIdx.x - 64; idx < KT * NS * 8; idx += 256) {
                     const int r = (idx >> 3) % KT;
-                    if (!((r < 32 ? lo : hi) >> (r & 31) & 1u))
-                        *reinterpret_cast<uint4*>(sV + st * Tc::K_TILE + (idx >> 3) / KT * Tc::K_SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t wd = r < 64 ? (r < 32 ? word[0] : word[1]) : (r < 96 ? word[2] : word[3]);
+                    if (!(wd >> (r & 31) & 1u)) *reinterpret_cast<uint4*>(sV + st * Tc::TILE + (idx >> 3) / KT * Tc::SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
             box = box_of(i + 1);
-            bad |= !wait_all(s_full + 8 * (i & 1), i >> 1, 11);
-            uint32_t p[16];
-            if (work) {
-                tc_fence_after();
+            bad |= !wait_all(s_full, i, 11);
+            // 32 scores of part p (cached rows [64 p, 64 p + 64) of the step), biased and masked
+            auto scores = [&](int p, float (&x)[32]) {
                 uint32_t r[32];
-                tmem_ld32(tmem + lanes + (i & 1) * 64 + half * 32, r);
+                tmem_ld32(tmem + lanes + p * 64 + half * 32, r);
                 tmem_ld_wait();
-                float x[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(r[j]);
                 if (a.alibi) {
-                    const float t0 = static_cast<float>(k.begin + i * KT + half * 32);
+                    const float f0 = far - static_cast<float>(t0 + p * 64 + half * 32);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = x[j] * a.c - slope * (far - (t0 + static_cast<float>(j)));
+                    for (int j = 0; j < 32; ++j) x[j] = x[j] * a.c - slope * (f0 - static_cast<float>(j));
                 }
                 if (!whole) {
-                    const uint32_t mask = half ? hi : lo;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) if (!(mask >> j & 1u)) x[j] = -INFINITY;
+                    for (int j = 0; j < 32; ++j) if (!(there[p] >> j & 1u)) x[j] = -INFINITY;
                 }
-                float top4[4] = {x[0], x[1], x[2], x[3]};
+            };
+            if (work) {
+                tc_fence_after();
+                float top = -INFINITY;
 #pragma unroll
-                for (int j = 4; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
-                float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * mul;
+                for (int p = 0; p < 2; ++p) {
+                    float x[32];
+                    scores(p, x);
+                    float top4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int j = 4; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
+                    top = fmaxf(top, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
+                }
+                top *= mul;
                 if (pair_any(quad, top > m + kAttnSlack || bad)) {
                     // rounded up: any point at or just above the maximum will do, and both threads take the same
                     const bf16 mine = __float2bfloat16_ru(top);
@@ -878,10 +904,11 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                     if (move) m = top;
                     l *= back;
                     if (i > 0) {
-                        bad |= !wait_all(pv_done, i - 1, 12);
+                        bad |= !wait_all(pv_done, 2 * i - 1, 12);
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DP / 2; c += 32) {
+                            uint32_t r[32];
                             tmem_ld32(tmem_o + lanes + half * (DP / 2) + c, r);
                             tmem_ld_wait();
 #pragma unroll
@@ -891,35 +918,49 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                         tmem_st_wait();
                     }
                 }
-                const float ref = m == -INFINITY ? 0.f : m;
-                const uint64_t mul_2 = pack2(mul, mul), ref_2 = pack2(-ref, -ref);
-                uint64_t sum0 = 0ull, sum1 = 0ull;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float e0, e1;
-                    unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul_2, ref_2), e0, e1);
-                    e0 = exp2_fast(e0);
-                    e1 = exp2_fast(e1);
-                    if (j & 1) sum1 = add2(sum1, pack2(e0, e1));
-                    else sum0 = add2(sum0, pack2(e0, e1));
-                    p[j] = pack_bf16x2(e0, e1);                 // rounded for the tensor cores, summed as they are
-                }
-                float s0, s1;
-                unpack2(add2(sum0, sum1), s0, s1);
-                l += s0 + s1;
             }
-            if (i > 0) bad |= !wait_all(pv_done, i - 1, 13);    // P of the step before is used up
-            if (work) {
+            const float ref = m == -INFINITY ? 0.f : m;
+            const uint64_t mul_2 = pack2(mul, mul), ref_2 = pack2(-ref, -ref);
+            uint64_t sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(prow + (((half * 4 + c) ^ sw) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
-            } else if (bad) break;
-            tc_fence_before();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            for (int p = 0; p < 2; ++p) {
+                uint32_t pk[16];
+                if (work) {
+                    float x[32];
+                    scores(p, x);
+                    if (p == 1) {                               // the scores are in registers: their columns go back to the tensor core
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_free);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float e0, e1;
+                        unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul_2, ref_2), e0, e1);
+                        e0 = exp2_fast(e0);
+                        e1 = exp2_fast(e1);
+                        if (j & 1) sum1 = add2(sum1, pack2(e0, e1));
+                        else sum0 = add2(sum0, pack2(e0, e1));
+                        pk[j] = pack_bf16x2(e0, e1);            // rounded for the tensor cores, summed as they are
+                    }
+                } else if (p == 1 && lane == 0) mbar_arrive(s_free);
+                if (i + p > 0) bad |= !wait_all(pv_done, 2 * i + p - 1, 13);      // the P before has been used
+                if (work) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(prow + (((half * 4 + c) ^ sw) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+                }
+                tc_fence_before();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full);
+            }
+            float s0, s1;
+            unpack2(add2(sum0, sum1), s0, s1);
+            l += s0 + s1;
+            if (!work && bad) break;
         }
         if (work) {
-            bad |= !wait_all(pv_done, steps - 1, 14);
+            bad |= !wait_all(pv_done, 2 * steps - 1, 14);
             sL[half * 128 + row] = l;
             if (!pair_any(quad, bad)) {
                 l += sL[(half ^ 1) * 128 + row];
