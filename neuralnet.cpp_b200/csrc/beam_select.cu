@@ -3,7 +3,7 @@
 // the n best, best first; equal values go to the lower (b, v).
 // Which of two continuations is better decides what a program answers.  A score and a logit are exact and values are compared
 // in 64 bits; the normaliser, the only rounded part, is summed in 64 bits from exponentials in 32, off by less than 1.5e-6 of
-// one (ex2 2^-22, its argument 2^-24 of about 10 twice, eight additions in 32 bits), most often by less than 1e-7.  Where
+// one (ex2 2^-22, its argument 2^-24 of about 10 twice, six additions in 32 bits), most often by less than 1e-7.  Where
 // continuations of two beams come closer than that, which happens to one group in some hundreds, their beams' normalisers
 // are computed again in 64 bits, as sums of whole numbers: exact to 1e-12, and the same in whatever order a row holds its logits.
 //
@@ -16,11 +16,12 @@
 
 #include "common.cuh"
 #include "nnb200.h"
+#include "tc_ptx.cuh"
 
 namespace nnb {
 
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32;
-constexpr int kSelPer = 16, kSelTile = kSelThreads * kSelPer;   // logits of a thread, and of the block, at a time
+constexpr int kSelThreads = 128, kSelWarps = kSelThreads / 32;  // few warps: what a block does besides its logits is done by each
+constexpr int kSelPer = 32, kSelTile = kSelThreads * kSelPer;   // logits of a thread, and of the block, at a time
 constexpr int kSelMost = 128;                                   // continuations of a group
 constexpr int kSelSlack = 256;                                  // a list this much longer than n is cut back to n
 constexpr int kSelList = kSelTile + kSelMost + kSelSlack;       // a tile may go into the list whole
@@ -45,39 +46,53 @@ __device__ __forceinline__ uint32_t order_of(float x)
     const uint32_t b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float exp_against(float x, float ref)
+__device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
+__device__ __forceinline__ float exp2_approx(float x)
 {
-    // (x - ref) log2(e), the constant in two parts: its rounding alone would move sums by 1e-7
-    const float d = x - ref;
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, 1.4426950216293335f, d * 1.925963033500e-8f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// exponentials of eight values against a reference point, added up: the argument is (x - ref) log2(e) with the constant in two
+// parts, because its rounding alone would move sums by 1e-7
+__device__ __forceinline__ float exps_against(const float* v, uint64_t minus_ref)
+{
+    const uint64_t hi = pack2(1.4426950216293335f, 1.4426950216293335f), lo = pack2(1.925963033500e-8f, 1.925963033500e-8f);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const uint64_t d = add2(pack2(v[j], v[j + 1]), minus_ref);
+        float x, y;
+        unpack2(fma2(d, hi, mul2(d, lo)), x, y);
+        const uint64_t e = pack2(exp2_approx(x), exp2_approx(y));
+        sum = j ? add2(sum, e) : e;
+    }
+    float x, y;
+    unpack2(sum, x, y);
+    return x + y;
+}
 
-// A bound that at least `want` of the threads' values reach, none of them counted twice: of each warp the k-th largest value for
-// k = want / 8 and want / 4, of the warps the smallest of the one, and the fourth of the other.  0 where there are too few.
+// A bound that at least `want` (up to 128) of the threads' values reach: of each of the W warps the k-th largest value, for
+// k = want / W the smallest of the warps', for k = 2 want / W the (W / 2)-th largest.  0 where there are too few.
+template <int W>
 __device__ __forceinline__ uint32_t bound_for(uint32_t mine, int want, uint32_t (*sw)[2])
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k8 = (want + 7) / 8, k4 = (want + 3) / 4;
-    uint32_t at8 = 0, top = 0;
-    for (int k = 1; k <= k4; ++k) {
+    static_assert(W >= 4 && W <= 32 && 128 / W <= 32, "a warp has that many values");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, all = (want + W - 1) / W, half = (2 * want + W - 1) / W, rounds = min(half, 32);
+    uint32_t at = 0, top = 0;
+    for (int k = 1; k <= rounds; ++k) {
         top = __reduce_max_sync(0xffffffffu, mine);
         const uint32_t who = __ballot_sync(0xffffffffu, mine == top);
         if (lane == __ffs(who) - 1) mine = 0;
-        if (k == k8) at8 = top;
+        if (k == all) at = top;
     }
-    if (lane == 0) { sw[warp][0] = at8; sw[warp][1] = top; }
+    if (lane == 0) { sw[warp][0] = at; sw[warp][1] = rounds == half ? top : 0; }
     __syncthreads();
-    uint32_t least = 0xffffffffu, fourth = 0;
+    const uint32_t least = __reduce_min_sync(0xffffffffu, lane < W ? sw[lane][0] : 0xffffffffu), h = lane < W ? sw[lane][1] : 0;
+    int above = 0;
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) {
-        least = min(least, sw[w][0]);
-        int above = 0;
-#pragma unroll
-        for (int v = 0; v < kSelWarps; ++v) above += sw[v][1] > sw[w][1] || (sw[v][1] == sw[w][1] && v < w) ? 1 : 0;
-        if (above == 3) fourth = sw[w][1];
-    }
-    return max(least, fourth);
+    for (int w = 0; w < W; ++w) { const uint32_t o = __shfl_sync(0xffffffffu, h, w); above += o > h || (o == h && w < lane) ? 1 : 0; }
+    return max(least, __reduce_max_sync(0xffffffffu, lane < W && above == W / 2 - 1 ? h : 0));
 }
 
 // a list entry: order of the value above, complement of the token below, so that the larger one is the better
@@ -103,12 +118,12 @@ __device__ int cut_list(SelectShared& sh, int n)
         constexpr int PER = (kSelList + kSelThreads - 1) / kSelThreads;
         Entry top = 0;
         for (int i = threadIdx.x; i < count; i += kSelThreads) top = max(top, sh.list[i]);
-        Entry bound = static_cast<Entry>(bound_for(static_cast<uint32_t>(top >> 32), n, sh.sw)) << 32;
+        Entry bound = static_cast<Entry>(bound_for<kSelWarps>(static_cast<uint32_t>(top >> 32), n, sh.sw)) << 32;
         // entries equal to the bound in value may be many: of those a bound of tokens
         uint32_t tie = 0;
         for (int i = threadIdx.x; i < count; i += kSelThreads) { const Entry e = sh.list[i]; if (e >> 32 == bound >> 32) tie = max(tie, static_cast<uint32_t>(e)); }
         __syncthreads();
-        bound |= bound_for(tie, n, sh.sw);
+        bound |= bound_for<kSelWarps>(tie, n, sh.sw);
         uint32_t keep = 0;
 #pragma unroll 1
         for (int j = 0; j < PER; ++j) {
@@ -137,6 +152,7 @@ __device__ int cut_list(SelectShared& sh, int n)
     for (int i = threadIdx.x; i < count; i += kSelThreads) {
         const Entry e = sh.list[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < count; ++j) rank += sh.list[j] > e;
         if (rank < n) sh.best[rank] = e;
     }
@@ -161,19 +177,28 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     constexpr int N = Vec16<T>::N, VECS = kSelPer / N;
-    float ref = -INFINITY;                                      // this thread's exponentials are taken against ref, near its maximum
+    // exponentials are taken against the first tile's maximum, or one of this thread's own where that is far behind
+    float ref = -INFINITY;
     double sum = 0.0;
-    uint32_t floor_ = 0;                                        // order of a value that n others reach: equal ones come too late
+    float least = 0.f;                                          // what can still be among the n best
+    int left = -1;                                              // entries of the list when it was cut last: all of them, sorted, if no more came
+    // whole tiles of aligned rows are read a tile ahead
+    Vec16<T> raw[VECS];
+    auto whole = [&](int t0) { return a.vectors && t0 + kSelTile <= end; };
+    auto ahead = [&](int t0) {
+        if (!whole(t0)) return;
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) raw[i] = ld16(x + t0 + (i * kSelThreads + static_cast<int>(threadIdx.x)) * N);
+    };
+    ahead(begin);
     for (int t0 = begin; t0 < end; t0 += kSelTile) {
         float v[kSelPer];
         // logit j of this thread is token_of(j): vectors of neighbours lie side by side
         auto token_of = [&](int j) { return a.vectors ? t0 + (j / N * kSelThreads + static_cast<int>(threadIdx.x)) * N + j % N : t0 + j * kSelThreads + static_cast<int>(threadIdx.x); };
-        if (a.vectors && t0 + kSelTile <= end) {
-            Vec16<T> r[VECS];
+        if (whole(t0)) {
 #pragma unroll
-            for (int i = 0; i < VECS; ++i) r[i] = ld16(x + token_of(i * N));
-#pragma unroll
-            for (int j = 0; j < kSelPer; ++j) v[j] = to_f32(r[j / N].v[j % N]);
+            for (int j = 0; j < kSelPer; ++j) v[j] = to_f32(raw[j / N].v[j % N]);
+            ahead(t0 + kSelTile);
         } else {
 #pragma unroll
             for (int j = 0; j < kSelPer; ++j) { const int t = token_of(j); v[j] = t < end ? to_f32(x[t]) : -INFINITY; }
@@ -181,39 +206,51 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < kSelPer; ++j) top = fmaxf(top, v[j]);
-        if (top > ref + 8.0f) { sum *= ref == -INFINITY ? 0.0 : exp(static_cast<double>(ref) - top); ref = top; }
-        const float r = ref == -INFINITY ? 0.f : ref;
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int j = 0; j < kSelPer; j += 2) { s0 += exp_against(v[j], r); s1 += exp_against(v[j + 1], r); }
-        sum += static_cast<double>(s0 + s1);
         const bool first = t0 == begin;
-        uint32_t least = floor_ + 1;
-        if (first) least = max(bound_for(order_of(top), a.n, sh.sw), order_of(-INFINITY) + 1);
-        if (order_of(top) >= least) {
+        if (first) {
+            ref = warp_max(top);
+            if (lane == 0) sh.ref[warp] = ref;
+            least = value_of(max(bound_for<kSelWarps>(order_of(top), a.n, sh.sw), order_of(-INFINITY) + 1));
+#pragma unroll
+            for (int w = 0; w < kSelWarps; ++w) ref = fmaxf(ref, sh.ref[w]);
+        }
+        if (top > ref + 64.0f) { sum *= ref == -INFINITY ? 0.0 : exp(static_cast<double>(ref) - top); ref = top; }
+        const float r = ref == -INFINITY ? 0.f : -ref;
+        const uint64_t minus_ref = pack2(r, r);
+        float part[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) part[h] = exps_against(v + 8 * h, minus_ref);
+        sum += static_cast<double>((part[0] + part[1]) + (part[2] + part[3]));
+        if (top >= least) {
+            int more = 0;
+#pragma unroll
+            for (int j = 0; j < kSelPer; ++j) more += v[j] >= least ? 1 : 0;
+            int at = atomicAdd(&sh.count, more);
 #pragma unroll
             for (int j = 0; j < kSelPer; ++j)
-                if (order_of(v[j]) >= least && v[j] == v[j]) sh.list[atomicAdd(&sh.count, 1)] = entry_of(v[j], token_of(j));
+                if (v[j] >= least) sh.list[at++] = entry_of(v[j], token_of(j));
         }
         __syncthreads();
         const int count = sh.count;
         if (first || count > a.n + kSelSlack) {
-            if (cut_list(sh, a.n) == a.n) floor_ = static_cast<uint32_t>(sh.list[a.n - 1] >> 32);
-            else floor_ = order_of(-INFINITY);
+            // from the n-th best up, but not equal to it: an equal one comes later in the row
+            left = cut_list(sh, a.n);
+            least = value_of((left == a.n ? static_cast<uint32_t>(sh.list[a.n - 1] >> 32) : order_of(-INFINITY)) + 1);
         }
-        __syncthreads();
+        if (t0 + kSelTile < end) __syncthreads();
     }
     // the block's sum, against the largest of the threads' points
     float m = ref;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) sh.ref[warp] = m;
-    const int left = cut_list(sh, a.n);
+    __syncthreads();
+    if (sh.count != left) left = cut_list(sh, a.n);
     m = sh.ref[0];
 #pragma unroll
     for (int w = 1; w < kSelWarps; ++w) m = fmaxf(m, sh.ref[w]);
     // a thread without a finite value adds what it has: 0, or NaN where there was one
-    double s = ref == -INFINITY ? sum : sum * exp(static_cast<double>(ref) - m);
+    double s = ref == -INFINITY || ref == m ? sum : sum * exp(static_cast<double>(ref) - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) sh.sum[warp] = s;
@@ -234,28 +271,36 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------- picking
-struct Cand { double value; int at, beam; };                    // at: beam * vocab + token
-__device__ __forceinline__ bool better(const Cand& x, const Cand& y) { return x.value > y.value || (x.value == y.value && x.at < y.at); }
-constexpr int kPickList = 2048;
+// order of doubles as order of unsigned numbers; at: beam * vocab + token
+struct Cand { unsigned long long key; int at, beam; };
+__device__ __forceinline__ unsigned long long order_of(double x)
+{
+    const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double value_of(unsigned long long order) { return __longlong_as_double(static_cast<long long>(order >> 63 ? order & ~(1ull << 63) : ~order)); }
+__device__ __forceinline__ bool better(const Cand& x, const Cand& y) { return x.key > y.key || (x.key == y.key && x.at < y.at); }
+constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32, kPickList = 2048;
 constexpr double kNear = 4e-6;                                  // values of two beams this close are compared again, exactly
 
 struct PickShared {
     double norm[64];            // log-sum-exp of each beam; NaN: its logits offer nothing
-    Cand list[kPickList];
-    uint32_t sw[kSelWarps][2];
-    Cand red[kSelWarps], last;
-    unsigned long long part[kSelWarps], again;                  // again: beams whose normalisers have to be exact
-    int count;
+    float score[64];
+    Cand list[kPickList], best[kSelMost];
+    uint32_t sw[kPickWarps][2];
+    Cand red[kPickWarps], last;
+    unsigned long long part[kPickWarps], again;                  // again: beams whose normalisers have to be exact
+    int count, ended[64];
 };
 
-__device__ __forceinline__ void put(const SelectArgs& a, int g, int k, const Cand& c)
+__device__ __forceinline__ void put(const SelectArgs& a, const PickShared& sh, int g, int k, const Cand& c)
 {
-    const bool none = !(c.value > -INFINITY);
+    const bool none = c.key == 0;
     const int to = g * a.n + k, token = none ? -1 : c.at - c.beam * a.vocab;
     a.parent[to] = none ? -1 : c.beam;
     a.token[to] = token;
-    a.scores_out[to] = none ? -INFINITY : static_cast<float>(c.value);
-    if (a.ended_out) a.ended_out[to] = !none && ((a.ended && a.ended[g * a.beams + c.beam]) || token == a.eos) ? 1 : 0;
+    a.scores_out[to] = none ? -INFINITY : static_cast<float>(value_of(c.key));
+    if (a.ended_out) a.ended_out[to] = !none && (sh.ended[c.beam] || token == a.eos) ? 1 : 0;
 }
 
 // log-sum-exp of a row whose sum is finite, by the whole block: exponentials in 64 bits, added as multiples of 2^-shift, 62 bits in all
@@ -268,7 +313,8 @@ __device__ double exact_norm(const SelectArgs& a, PickShared& sh, int row)
     for (int i = 0; i < a.spans; ++i) { const int2 e = a.list[(static_cast<long long>(row) * a.spans + i) * a.n]; if (e.y >= 0) m = fmaxf(m, __int_as_float(e.x)); }
     const double scale = static_cast<double>(1ull << shift);
     unsigned long long sum = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kSelThreads) sum += __double2ull_rn(exp(static_cast<double>(to_f32(x[i])) - m) * scale);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.vocab; i += kPickThreads) sum += __double2ull_rn(exp(static_cast<double>(to_f32(x[i])) - m) * scale);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     __syncthreads();
@@ -276,97 +322,134 @@ __device__ double exact_norm(const SelectArgs& a, PickShared& sh, int row)
     __syncthreads();
     sum = 0;
 #pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) sum += sh.part[w];
+    for (int w = 0; w < kPickWarps; ++w) sum += sh.part[w];
     return static_cast<double>(m) + log(static_cast<double>(sum) / scale);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSelThreads) select_pick_kernel(const __grid_constant__ SelectArgs a)
+__global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_constant__ SelectArgs a)
 {
     __shared__ PickShared sh;
     const int g = static_cast<int>(blockIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // written before the kernel in front of this one began
+    if (static_cast<int>(threadIdx.x) < a.beams) {
+        sh.score[threadIdx.x] = a.scores[g * a.beams + threadIdx.x];
+        sh.ended[threadIdx.x] = a.ended ? a.ended[g * a.beams + threadIdx.x] : 0;
+    }
+    if (threadIdx.x == 0) { sh.count = 0; sh.again = 0; }
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int b = warp; b < a.beams; b += kSelWarps) {           // a warp per beam
-        const int row = g * a.beams + b;
-        if (a.ended && a.ended[row]) { if (lane == 0) sh.norm[b] = NAN; continue; }
-        const SpanSum* st = a.stat + static_cast<long long>(row) * a.spans;
+    // candidate i: the rows' lists side by side, best entries first, then the ended beams' own.  A thread's candidates are then of
+    // like places in different lists, and the best of each list with different threads: what the bound below lives on.
+    const int rows = a.beams * a.spans, lists = rows * a.n, all = lists + a.beams;
+    const Cand nothing{0, INT_MAX, -1};
+    struct Raw { int2 e; int beam; };
+    auto raw = [&](int i) -> Raw {
+        if (i >= lists) return {make_int2(0, a.eos), i - lists};
+        const int k = i / rows, r = i - k * rows, b = r / a.spans;
+        if (sh.ended[b]) return {make_int2(0, -1), b};          // its lists were not written
+        return {a.list[(static_cast<long long>(g) * rows + r) * a.n + k], b};
+    };
+    auto cand = [&](int i, const Raw& w) -> Cand {
+        double v = sh.score[w.beam];
+        if (i >= lists) { if (!sh.ended[w.beam]) return nothing; }
+        else {
+            if (w.e.y < 0) return nothing;
+            v += static_cast<double>(__int_as_float(w.e.x)) - sh.norm[w.beam];
+        }
+        return v > -INFINITY ? Cand{order_of(v), w.beam * a.vocab + w.e.y, w.beam} : nothing;
+    };
+    const int first = threadIdx.x;
+    Raw mine_raw{make_int2(0, -1), 0};
+    if (first < all) mine_raw = raw(first);
+    for (int b = warp; b < a.beams; b += kPickWarps) {           // a warp per beam
+        if (sh.ended[b]) { if (lane == 0) sh.norm[b] = NAN; continue; }
+        const SpanSum* st = a.stat + static_cast<long long>(g * a.beams + b) * a.spans;
         float m = -INFINITY;
         for (int i = lane; i < a.spans; i += 32) m = fmaxf(m, st[i].ref);
         m = warp_max(m);
         double s = 0.0;
-        for (int i = lane; i < a.spans; i += 32) s += st[i].ref == -INFINITY ? st[i].sum : st[i].sum * exp(static_cast<double>(st[i].ref) - m);
+        for (int i = lane; i < a.spans; i += 32) s += st[i].ref == -INFINITY ? st[i].sum : (st[i].ref == m ? st[i].sum : st[i].sum * exp(static_cast<double>(st[i].ref) - m));
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         // NaN from a NaN or +inf logit; a row of -inf has no maximum
         if (lane == 0) sh.norm[b] = m == -INFINITY ? static_cast<double>(NAN) : static_cast<double>(m) + log(s);
     }
-    if (threadIdx.x == 0) { sh.count = 0; sh.again = 0; }
     __syncthreads();
-    const int per = a.spans * a.n, lists = a.beams * per, all = lists + a.beams;
-    const Cand nothing{-INFINITY, INT_MAX, -1};
-    // candidate i: the entries of the beams' lists, then the ended beams' own
-    auto cand = [&](int i) -> Cand {
-        if (i < lists) {
-            const int b = i / per;
-            const double norm = sh.norm[b];
-            if (norm != norm) return nothing;                   // also where the lists were not written
-            const int2 e = a.list[static_cast<long long>(g) * lists + i];
-            if (e.y < 0) return nothing;
-            const double v = static_cast<double>(a.scores[g * a.beams + b]) + (static_cast<double>(__int_as_float(e.x)) - norm);
-            return v > -INFINITY ? Cand{v, b * a.vocab + e.y, b} : nothing;
-        }
-        const int b = i - lists;
-        if (!a.ended || !a.ended[g * a.beams + b]) return nothing;
-        const double v = a.scores[g * a.beams + b];
-        return v > -INFINITY ? Cand{v, b * a.vocab + a.eos, b} : nothing;
-    };
     // a value that n candidates reach, in 32 bits (rounding keeps the order but for equality), and by kNear less once normalisers move
-    uint32_t top = 0;
-    for (int i = threadIdx.x; i < all; i += kSelThreads) {
-        const Cand x = cand(i);
-        if (x.value > -INFINITY) top = max(top, order_of(static_cast<float>(x.value)));
+    Cand mine = first < all ? cand(first, mine_raw) : nothing;
+    uint32_t top = mine.key ? order_of(static_cast<float>(value_of(mine.key))) : 0;
+    for (int i = first + kPickThreads; i < all; i += kPickThreads) {
+        const Cand x = cand(i, raw(i));
+        if (x.key) top = max(top, order_of(static_cast<float>(value_of(x.key))));
     }
-    const uint32_t key = bound_for(top, a.n, sh.sw);
-    double bound = -INFINITY;
-    if (key) {
-        const float b = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-        bound = static_cast<double>(b) - fabs(static_cast<double>(b)) * 0x1p-23 - 2.0 * kNear;
-        if (!(bound > -INFINITY)) bound = b == INFINITY ? 3e38 : -INFINITY;
-    }
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int i = threadIdx.x; i < all; i += kSelThreads) {
-            const Cand x = cand(i);
-            if (x.value > -INFINITY && x.value >= bound) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kPickList) sh.list[at] = x;
-            }
+    const uint32_t key = bound_for<kPickWarps>(top, a.n, sh.sw);
+    auto below = [](uint32_t k) -> unsigned long long {
+        if (k == 0) return 1;
+        const double b = value_of(k), less = b - fabs(b) * 0x1p-23 - 2.0 * kNear;
+        return b == INFINITY ? order_of(3e38) : (less > -INFINITY ? order_of(less) : 1);
+    };
+    const unsigned long long bound = below(key);
+    auto add = [&](const Cand& x) {
+        if (x.key >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kPickList) sh.list[at] = x;
         }
+    };
+    for (int pass = 0; pass < 2; ++pass) {
+        if (pass == 1 && first < all) mine = cand(first, mine_raw);
+        add(mine);
+        for (int i = first + kPickThreads; i < all; i += kPickThreads) add(cand(i, raw(i)));
         __syncthreads();
-        const int count = sh.count;
+        int count = sh.count;
+        // a long list is thinned: with its entries spread over the threads a bound leaves little more than n
+        for (int round = 0; round < 2 && count > a.n + 256 && count <= kPickList; ++round) {
+            uint32_t most = 0;
+            for (int i = threadIdx.x; i < count; i += kPickThreads) most = max(most, order_of(static_cast<float>(value_of(sh.list[i].key))));
+            const unsigned long long tight = below(bound_for<kPickWarps>(most, a.n, sh.sw));
+            Cand kept[kPickList / kPickThreads];
+#pragma unroll
+            for (int j = 0; j < kPickList / kPickThreads; ++j) {
+                const int i = threadIdx.x + j * kPickThreads;
+                kept[j] = i < count && sh.list[i].key >= tight ? sh.list[i] : nothing;
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) sh.count = 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kPickList / kPickThreads; ++j) if (kept[j].key) sh.list[atomicAdd(&sh.count, 1)] = kept[j];
+            __syncthreads();
+            count = sh.count;
+            __syncthreads();
+        }
         if (count > kPickList) {
-            if (pass == 0 && threadIdx.x == 0) sh.again = ~0ull;
+            if (threadIdx.x == 0) sh.again = ~0ull;
         } else {
-            for (int i = threadIdx.x; i < count; i += kSelThreads) {
+            // what is close to one of the n best may belong before it, and its beam's normaliser has to be exact too
+            for (int i = threadIdx.x; i < count; i += kPickThreads) {
                 const Cand x = sh.list[i];
+                const unsigned long long under = order_of(value_of(x.key) - kNear), over = order_of(value_of(x.key) + kNear);
                 int rank = 0;
                 unsigned long long near = 0;
+#pragma unroll 4
                 for (int j = 0; j < count; ++j) {
                     const Cand y = sh.list[j];
                     rank += better(y, x);
-                    if (y.beam != x.beam && fabs(y.value - x.value) < kNear) near |= 1ull << y.beam | 1ull << x.beam;
+                    if (y.key > under && y.key < over && y.beam != x.beam) near |= 1ull << y.beam | 1ull << x.beam;
                 }
                 if (rank < a.n) {
+                    sh.best[rank] = x;
                     if (pass == 0 && near) atomicOr(&sh.again, near);
-                    put(a, g, rank, x);
                 }
             }
-            for (int k = count + threadIdx.x; k < a.n; k += kSelThreads) put(a, g, k, nothing);
+            for (int k = count + threadIdx.x; k < a.n; k += kPickThreads) sh.best[k] = nothing;
         }
         __syncthreads();
         const unsigned long long again = sh.again;
-        if (pass == 1 || again == 0) {
-            if (count <= kPickList) return;
-            break;
+        if (count <= kPickList && (pass == 1 || again == 0)) {
+            for (int k = threadIdx.x; k < a.n; k += kPickThreads) put(a, sh, g, k, sh.best[k]);
+            return;
         }
+        if (pass == 1) break;
         if (threadIdx.x == 0) sh.count = 0;
         for (int b = 0; b < a.beams; ++b) {
             const double norm = sh.norm[b];
@@ -378,26 +461,26 @@ __global__ void __launch_bounds__(kSelThreads) select_pick_kernel(const __grid_c
         __syncthreads();
     }
     // more candidates near the bound than the list takes: one place at a time
-    if (threadIdx.x == 0) sh.last = {INFINITY, -1, -1};
+    if (threadIdx.x == 0) sh.last = {~0ull, -1, -1};
     __syncthreads();
     for (int k = 0; k < a.n; ++k) {
         const Cand prev = sh.last;
         Cand best = nothing;
-        for (int i = threadIdx.x; i < all; i += kSelThreads) {
-            const Cand x = cand(i);
-            if (x.value > -INFINITY && better(prev, x) && better(x, best)) best = x;
+        for (int i = threadIdx.x; i < all; i += kPickThreads) {
+            const Cand x = cand(i, raw(i));
+            if (x.key && better(prev, x) && better(x, best)) best = x;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            const Cand x{__shfl_xor_sync(0xffffffffu, best.value, o), __shfl_xor_sync(0xffffffffu, best.at, o), __shfl_xor_sync(0xffffffffu, best.beam, o)};
+            const Cand x{__shfl_xor_sync(0xffffffffu, best.key, o), __shfl_xor_sync(0xffffffffu, best.at, o), __shfl_xor_sync(0xffffffffu, best.beam, o)};
             if (better(x, best)) best = x;
         }
         if (lane == 0) sh.red[warp] = best;
         __syncthreads();
         if (threadIdx.x == 0) {
-            for (int w = 1; w < kSelWarps; ++w) if (better(sh.red[w], best)) best = sh.red[w];
+            for (int w = 1; w < kPickWarps; ++w) if (better(sh.red[w], best)) best = sh.red[w];
             sh.last = best;
-            put(a, g, k, best);
+            put(a, sh, g, k, best);
         }
         __syncthreads();
     }
@@ -418,7 +501,7 @@ template <typename T> static int select_t(SelectArgs a, cudaStream_t s)
     NNB_LAUNCH_CHECK();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.groups));
-    cfg.blockDim = dim3(kSelThreads);
+    cfg.blockDim = dim3(kPickThreads);
     cfg.stream = s;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
