@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
     // exponentials are taken against the first tile's maximum, or one of this thread's own where that is far behind
     float ref = -INFINITY;
     double sum = 0.0;
-    float least = 0.f;                                          // what can still be among the n best
+    float most = -INFINITY, least = 0.f;                        // the thread's maximum; what can still be among the n best
     int left = -1;                                              // entries of the list when it was cut last: all of them, sorted, if no more came
     // whole tiles of aligned rows are read a tile ahead
     Vec16<T> raw[VECS];
@@ -222,14 +222,18 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
         for (int h = 0; h < 4; ++h) part[h] = exps_against(v + 8 * h, minus_ref);
         sum += static_cast<double>((part[0] + part[1]) + (part[2] + part[3]));
         if (top >= least) {
-            int more = 0;
+            // few of a warp's logits get here, and not often: they are read again, by number
+            uint32_t hits = 0;
 #pragma unroll
-            for (int j = 0; j < kSelPer; ++j) more += v[j] >= least ? 1 : 0;
-            int at = atomicAdd(&sh.count, more);
-#pragma unroll
-            for (int j = 0; j < kSelPer; ++j)
-                if (v[j] >= least) sh.list[at++] = entry_of(v[j], token_of(j));
+            for (int j = 0; j < kSelPer; ++j) hits |= v[j] >= least ? 1u << j : 0u;
+            int at = atomicAdd(&sh.count, __popc(hits));
+            for (; hits; hits &= hits - 1) { const int t = token_of(__ffs(hits) - 1); sh.list[at++] = entry_of(to_f32(x[t]), t); }
         }
+        // thread maxima so far bound what is to come; worth its time when twice as much has been seen
+        most = fmaxf(most, top);
+        const int seen = (t0 - begin) / kSelTile + 1;
+        uint32_t bound = 0;
+        if (!first && (seen & (seen - 1)) == 0 && t0 + kSelTile < end) bound = bound_for<kSelWarps>(order_of(most), a.n, sh.sw);
         __syncthreads();
         const int count = sh.count;
         if (first || count > a.n + kSelSlack) {
@@ -237,6 +241,7 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
             left = cut_list(sh, a.n);
             least = value_of((left == a.n ? static_cast<uint32_t>(sh.list[a.n - 1] >> 32) : order_of(-INFINITY)) + 1);
         }
+        if (bound) least = fmaxf(least, value_of(bound + 1));
         if (t0 + kSelTile < end) __syncthreads();
     }
     // the block's sum, against the largest of the threads' points
@@ -280,20 +285,21 @@ __device__ __forceinline__ unsigned long long order_of(double x)
 }
 __device__ __forceinline__ double value_of(unsigned long long order) { return __longlong_as_double(static_cast<long long>(order >> 63 ? order & ~(1ull << 63) : ~order)); }
 __device__ __forceinline__ bool better(const Cand& x, const Cand& y) { return x.key > y.key || (x.key == y.key && x.at < y.at); }
-constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32, kPickList = 2048;
+constexpr int kPickList = 2048;
 constexpr double kNear = 4e-6;                                  // values of two beams this close are compared again, exactly
 
-struct PickShared {
+template <int W> struct PickShared {
     double norm[64];            // log-sum-exp of each beam; NaN: its logits offer nothing
     float score[64];
     Cand list[kPickList], best[kSelMost];
-    uint32_t sw[kPickWarps][2];
-    Cand red[kPickWarps], last;
-    unsigned long long part[kPickWarps], again;                  // again: beams whose normalisers have to be exact
+    uint32_t sw[W][2];
+    Cand red[W], last;
+    unsigned long long part[W], again;                  // again: beams whose normalisers have to be exact
     int count, ended[64];
 };
 
-__device__ __forceinline__ void put(const SelectArgs& a, const PickShared& sh, int g, int k, const Cand& c)
+template <int W>
+__device__ __forceinline__ void put(const SelectArgs& a, const PickShared<W>& sh, int g, int k, const Cand& c)
 {
     const bool none = c.key == 0;
     const int to = g * a.n + k, token = none ? -1 : c.at - c.beam * a.vocab;
@@ -304,8 +310,8 @@ __device__ __forceinline__ void put(const SelectArgs& a, const PickShared& sh, i
 }
 
 // log-sum-exp of a row whose sum is finite, by the whole block: exponentials in 64 bits, added as multiples of 2^-shift, 62 bits in all
-template <typename T>
-__device__ double exact_norm(const SelectArgs& a, PickShared& sh, int row)
+template <typename T, int W>
+__device__ double exact_norm(const SelectArgs& a, PickShared<W>& sh, int row)
 {
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, shift = 62 - (32 - __clz(a.vocab));
@@ -314,7 +320,7 @@ __device__ double exact_norm(const SelectArgs& a, PickShared& sh, int row)
     const double scale = static_cast<double>(1ull << shift);
     unsigned long long sum = 0;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < a.vocab; i += kPickThreads) sum += __double2ull_rn(exp(static_cast<double>(to_f32(x[i])) - m) * scale);
+    for (int i = threadIdx.x; i < a.vocab; i += (W * 32)) sum += __double2ull_rn(exp(static_cast<double>(to_f32(x[i])) - m) * scale);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     __syncthreads();
@@ -322,14 +328,14 @@ __device__ double exact_norm(const SelectArgs& a, PickShared& sh, int row)
     __syncthreads();
     sum = 0;
 #pragma unroll
-    for (int w = 0; w < kPickWarps; ++w) sum += sh.part[w];
+    for (int w = 0; w < W; ++w) sum += sh.part[w];
     return static_cast<double>(m) + log(static_cast<double>(sum) / scale);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_constant__ SelectArgs a)
+template <typename T, int W>
+__global__ void __launch_bounds__(W * 32) select_pick_kernel(const __grid_constant__ SelectArgs a)
 {
-    __shared__ PickShared sh;
+    __shared__ PickShared<W> sh;
     const int g = static_cast<int>(blockIdx.x), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // written before the kernel in front of this one began
     if (static_cast<int>(threadIdx.x) < a.beams) {
@@ -362,7 +368,7 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
     const int first = threadIdx.x;
     Raw mine_raw{make_int2(0, -1), 0};
     if (first < all) mine_raw = raw(first);
-    for (int b = warp; b < a.beams; b += kPickWarps) {           // a warp per beam
+    for (int b = warp; b < a.beams; b += W) {           // a warp per beam
         if (sh.ended[b]) { if (lane == 0) sh.norm[b] = NAN; continue; }
         const SpanSum* st = a.stat + static_cast<long long>(g * a.beams + b) * a.spans;
         float m = -INFINITY;
@@ -378,11 +384,11 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
     // a value that n candidates reach, in 32 bits (rounding keeps the order but for equality), and by kNear less once normalisers move
     Cand mine = first < all ? cand(first, mine_raw) : nothing;
     uint32_t top = mine.key ? order_of(static_cast<float>(value_of(mine.key))) : 0;
-    for (int i = first + kPickThreads; i < all; i += kPickThreads) {
+    for (int i = first + (W * 32); i < all; i += (W * 32)) {
         const Cand x = cand(i, raw(i));
         if (x.key) top = max(top, order_of(static_cast<float>(value_of(x.key))));
     }
-    const uint32_t key = bound_for<kPickWarps>(top, a.n, sh.sw);
+    const uint32_t key = bound_for<W>(top, a.n, sh.sw);
     auto below = [](uint32_t k) -> unsigned long long {
         if (k == 0) return 1;
         const double b = value_of(k), less = b - fabs(b) * 0x1p-23 - 2.0 * kNear;
@@ -398,25 +404,25 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
     for (int pass = 0; pass < 2; ++pass) {
         if (pass == 1 && first < all) mine = cand(first, mine_raw);
         add(mine);
-        for (int i = first + kPickThreads; i < all; i += kPickThreads) add(cand(i, raw(i)));
+        for (int i = first + (W * 32); i < all; i += (W * 32)) add(cand(i, raw(i)));
         __syncthreads();
         int count = sh.count;
         // a long list is thinned: with its entries spread over the threads a bound leaves little more than n
         for (int round = 0; round < 2 && count > a.n + 256 && count <= kPickList; ++round) {
             uint32_t most = 0;
-            for (int i = threadIdx.x; i < count; i += kPickThreads) most = max(most, order_of(static_cast<float>(value_of(sh.list[i].key))));
-            const unsigned long long tight = below(bound_for<kPickWarps>(most, a.n, sh.sw));
-            Cand kept[kPickList / kPickThreads];
+            for (int i = threadIdx.x; i < count; i += (W * 32)) most = max(most, order_of(static_cast<float>(value_of(sh.list[i].key))));
+            const unsigned long long tight = below(bound_for<W>(most, a.n, sh.sw));
+            Cand kept[kPickList / (W * 32)];
 #pragma unroll
-            for (int j = 0; j < kPickList / kPickThreads; ++j) {
-                const int i = threadIdx.x + j * kPickThreads;
+            for (int j = 0; j < kPickList / (W * 32); ++j) {
+                const int i = threadIdx.x + j * (W * 32);
                 kept[j] = i < count && sh.list[i].key >= tight ? sh.list[i] : nothing;
             }
             __syncthreads();
             if (threadIdx.x == 0) sh.count = 0;
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < kPickList / kPickThreads; ++j) if (kept[j].key) sh.list[atomicAdd(&sh.count, 1)] = kept[j];
+            for (int j = 0; j < kPickList / (W * 32); ++j) if (kept[j].key) sh.list[atomicAdd(&sh.count, 1)] = kept[j];
             __syncthreads();
             count = sh.count;
             __syncthreads();
@@ -424,29 +430,31 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
         if (count > kPickList) {
             if (threadIdx.x == 0) sh.again = ~0ull;
         } else {
-            // what is close to one of the n best may belong before it, and its beam's normaliser has to be exact too
-            for (int i = threadIdx.x; i < count; i += kPickThreads) {
-                const Cand x = sh.list[i];
+            // four threads an entry.  What is close to one of the n best may belong before it, and its beam's normaliser has
+            // to be exact too
+            for (int i = threadIdx.x >> 2; i < (count + 7) / 8 * 8; i += W * 8) {
+                const Cand x = sh.list[min(i, count - 1)];
                 const unsigned long long under = order_of(value_of(x.key) - kNear), over = order_of(value_of(x.key) + kNear);
                 int rank = 0;
                 unsigned long long near = 0;
-#pragma unroll 4
-                for (int j = 0; j < count; ++j) {
+                for (int j = threadIdx.x & 3; j < count; j += 4) {
                     const Cand y = sh.list[j];
                     rank += better(y, x);
                     if (y.key > under && y.key < over && y.beam != x.beam) near |= 1ull << y.beam | 1ull << x.beam;
                 }
-                if (rank < a.n) {
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) { rank += __shfl_xor_sync(0xffffffffu, rank, o); near |= __shfl_xor_sync(0xffffffffu, near, o); }
+                if (i < count && (threadIdx.x & 3) == 0 && rank < a.n) {
                     sh.best[rank] = x;
                     if (pass == 0 && near) atomicOr(&sh.again, near);
                 }
             }
-            for (int k = count + threadIdx.x; k < a.n; k += kPickThreads) sh.best[k] = nothing;
+            for (int k = count + threadIdx.x; k < a.n; k += (W * 32)) sh.best[k] = nothing;
         }
         __syncthreads();
         const unsigned long long again = sh.again;
         if (count <= kPickList && (pass == 1 || again == 0)) {
-            for (int k = threadIdx.x; k < a.n; k += kPickThreads) put(a, sh, g, k, sh.best[k]);
+            for (int k = threadIdx.x; k < a.n; k += (W * 32)) put(a, sh, g, k, sh.best[k]);
             return;
         }
         if (pass == 1) break;
@@ -454,7 +462,7 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
         for (int b = 0; b < a.beams; ++b) {
             const double norm = sh.norm[b];
             if (!(again >> b & 1ull) || norm != norm) continue;  // the same for all threads; an ended beam has no normaliser
-            const double exact = exact_norm<T>(a, sh, g * a.beams + b);
+            const double exact = exact_norm<T, W>(a, sh, g * a.beams + b);
             __syncthreads();
             if (threadIdx.x == 0) sh.norm[b] = exact;
         }
@@ -466,7 +474,7 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
     for (int k = 0; k < a.n; ++k) {
         const Cand prev = sh.last;
         Cand best = nothing;
-        for (int i = threadIdx.x; i < all; i += kPickThreads) {
+        for (int i = threadIdx.x; i < all; i += (W * 32)) {
             const Cand x = cand(i, raw(i));
             if (x.key && better(prev, x) && better(x, best)) best = x;
         }
@@ -478,7 +486,7 @@ __global__ void __launch_bounds__(kPickThreads) select_pick_kernel(const __grid_
         if (lane == 0) sh.red[warp] = best;
         __syncthreads();
         if (threadIdx.x == 0) {
-            for (int w = 1; w < kPickWarps; ++w) if (better(sh.red[w], best)) best = sh.red[w];
+            for (int w = 1; w < W; ++w) if (better(sh.red[w], best)) best = sh.red[w];
             sh.last = best;
             put(a, sh, g, k, best);
         }
@@ -501,14 +509,16 @@ template <typename T> static int select_t(SelectArgs a, cudaStream_t s)
     NNB_LAUNCH_CHECK();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.groups));
-    cfg.blockDim = dim3(kPickThreads);
+    // candidates on most threads: the bound is the n-th of the threads' best
+    const bool many = static_cast<long long>(a.beams) * a.spans * a.n > 1024;
+    cfg.blockDim = dim3(many ? 512 : 128);
     cfg.stream = s;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    NNB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, select_pick_kernel<T>, a));
+    NNB_CUDA_CHECK(many ? cudaLaunchKernelEx(&cfg, select_pick_kernel<T, 16>, a) : cudaLaunchKernelEx(&cfg, select_pick_kernel<T, 4>, a));
     NNB_LAUNCH_CHECK();
     return 0;
 }
