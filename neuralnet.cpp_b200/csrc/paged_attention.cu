@@ -726,6 +726,10 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DP >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     auto wait = [&](uint32_t bar, int parity, int code) -> bool { return mbar_wait(bar, parity & 1, abort_flag, code, &g_paged_attn_error); };
     auto wait_all = [&](uint32_t bar, int parity, int code) -> bool { return __all_sync(0xffffffffu, wait(bar, parity, code)); };
+    // whether a page of the run is missing: looked over once, by every warp for itself
+    bool gaps = false;
+    for (int t = k.begin + lane * high; t < k.end; t += 32 * high) gaps |= pool.find(k.table, k.hk, t) < 0;
+    gaps = __any_sync(0xffffffffu, gaps);
     // first row in the pool of the box this lane has of step i, -1: it is not there (the whole warp calls this)
     auto box_of = [&](int i) -> int {
         const int t = k.begin + i * KT + lane * high;
@@ -836,16 +840,15 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
         const float far = a.alibi && live ? static_cast<float>(far_of(a, pool.page_shift, k, w.seq)) : 0.f;
         float m = -INFINITY, l = 0.f;
         bool bad = *abort_flag != 0;                            // a wait of this thread gave up
-        int box = box_of(0);
         for (int i = 0; i < steps; ++i) {
             const int st = i % ST;
             // bit r of there[p]: row p * 64 + half * 32 + r of the step is there; all of them but for the last step and missing pages
-            const int t0 = k.begin + i * KT, count = box < 0 ? 0 : min(high, k.end - (t0 + lane * high));
-            const bool whole = __all_sync(0xffffffffu, lane >= boxes || count == high);
+            const int t0 = k.begin + i * KT;
+            const bool whole = !gaps && t0 + KT <= k.end;
             uint32_t there[2] = {0xffffffffu, 0xffffffffu};
             if (!whole) {
                 // rows [from, from + count) of the step are this lane's, as bits of its 128
-                const int from = lane * high;
+                const int from = lane * high, count = box_of(i) < 0 ? 0 : min(high, k.end - (t0 + from));
                 uint32_t word[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -861,7 +864,6 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                     if (!(wd >> (r & 31) & 1u)) *reinterpret_cast<uint4*>(sV + st * Tc::TILE + (idx >> 3) / KT * Tc::SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
-            box = box_of(i + 1);
             bad |= !wait_all(s_full, i, 11);
             // 32 scores of part p (cached rows [64 p, 64 p + 64) of the step), biased and masked
             auto scores = [&](int p, float (&x)[32]) {
@@ -1239,8 +1241,8 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     const long long rows = static_cast<long long>(size) * m;
     // fp32 tiles take 16 query rows; bf16 streams 8 or 16; beyond that tcgen05 tiles take 128, and where a head is too wide
     // for those mma.sync tiles take 64
-    p.tc = kv.dtype == 1 && rows > 16 && kv.head_dim <= 128 && prefix_stride > 0;
-    p.rt = kv.dtype == 0 ? 16 : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : 64)));
+    p.tc = kv.dtype == 1 && rows > 64 && kv.head_dim <= 128 && prefix_stride > 0;
+    p.rt = kv.dtype == 0 ? 16 : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 128 ? 32 : 64))));
     p.own_rows = p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
     p.row_tiles = static_cast<int>(ceil_div(rows, p.rt));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
@@ -1287,14 +1289,13 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
         };
         auto width = [&](auto dp) {
             constexpr int DP = decltype(dp)::value;
-            static PerDeviceOnce once[4];
+            static PerDeviceOnce once[6];
             if constexpr (sizeof(T) == 4) return go(paged_attn_f32_kernel<DP>, AttnTile32<DP>::SMEM, once[0]);
             else {
                 const bool wide = p.own_rows == 16;
-                if constexpr (DP == 256) {
-                    constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));
-                    if (p.rt == 64) return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[3]);
-                }
+                constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));
+                if (p.rt == 64) return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[3]);
+                if constexpr (DP < 256) if (p.rt == 32) return wide ? go(paged_attn_bf16_kernel<DP, 2, 2>, both, once[4]) : go(paged_attn_bf16_kernel<DP, 2, 1>, both, once[5]);
                 return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::smem(4), once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::smem(4), once[1]);
             }
         };
