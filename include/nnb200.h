@@ -517,6 +517,21 @@ int nnb200_beam_select(const void* logits, long long ld, int dtype, int groups, 
  * length, and every sequence pages of its own for the rows to come: with these, nothing that two sequences share is written. */
 int nnb200_beam_reorder(const nnb200_paged_kv* kv, int groups, int beams, const int32_t* parent, const int32_t* len, const int32_t* page_table,
                         const int32_t* spare, int32_t* len_out, int32_t* page_table_out, int32_t* spare_out, int table_stride, void* stream);
+/* Several continuations of one prompt through the model, a token of each at a time, over the above.  The prompt goes into the
+ * decode workspace first (nnb200_gpt_prefill); _begin copies its prompt_len rows into pages and gives every one of `seqs`
+ * (1..1024) sequences pages for new_rows rows of its own (prompt_len + new_rows <= seq).  _step runs token tokens[i] (device) of
+ * sequence i at its own row `step` (0, 1, .. new_rows - 1, the rows before it in place), position prompt_len + step, and writes
+ * (seqs, vocab) fp32 logits: what nnb200_gpt_forward_step gives for each sequence by itself.  _reorder makes sequence i's rows so
+ * far those of sequence parent[i] (device; out of range: its own).  The decode workspace is read by _begin, and by _step for its
+ * position tables.  workspace: _workspace_bytes bytes, 256-byte aligned, the caller's, with the same seqs and new_rows in
+ * every call; heads a multiple of 8 wide, up to 256. */
+long long nnb200_gpt_batch_workspace_bytes(const nnb200_gpt_config* cfg, int seqs, int new_rows);
+int nnb200_gpt_batch_begin(const nnb200_gpt_config* cfg, const void* decode_workspace, void* workspace, int seqs, int new_rows, int prompt_len,
+                           void* stream);
+int nnb200_gpt_batch_step(const nnb200_gpt_config* cfg, const float* params, const void* params_bf16, const void* decode_workspace,
+                          void* workspace, int seqs, int new_rows, int prompt_len, int step, const int32_t* tokens, float* logits_out,
+                          void* stream);
+int nnb200_gpt_batch_reorder(const nnb200_gpt_config* cfg, void* workspace, int seqs, int new_rows, const int32_t* parent, void* stream);
 
 #ifdef __cplusplus
 }

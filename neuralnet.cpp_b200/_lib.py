@@ -122,6 +122,10 @@ SIGNATURES = {
     "nnb200_beam_select_scratch_bytes": [_i, _i, _i, _i],
     "nnb200_beam_select": [_p, _ll, _i, _i, _i, _i, _p, _p, _i, _i, _p, _p, _p, _p, _p, _sz, _p],
     "nnb200_beam_reorder": [_kvp, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i, _p],
+    "nnb200_gpt_batch_workspace_bytes": [_cfgp, _i, _i],
+    "nnb200_gpt_batch_begin": [_cfgp, _p, _p, _i, _i, _i, _p],
+    "nnb200_gpt_batch_step": [_cfgp, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _p],
+    "nnb200_gpt_batch_reorder": [_cfgp, _p, _i, _i, _p, _p],
     # engine primitives in the reference's layouts
     "nnb200_batched_matmul": [_p, _p, _p, _sz, _sz, _sz, _sz, _u, _i, _i, _f, _p],
     "nnb200_bmm_reduce": [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p],
@@ -155,7 +159,7 @@ _RET = {
     "nnb200_muon_scratch_bytes": _sz, "nnb200_gpt_arena_elems": _ll, "nnb200_gpt_matrix_region_begin": _ll,
     "nnb200_gpt_layer_matrix_begin": _ll, "nnb200_gpt_workspace_bytes": _ll, "nnb200_gpt_workspace_offset": _ll,
     "nnb200_gpt_decode_workspace_bytes": _ll,
-    "nnb200_paged_attention_scratch_bytes": _sz, "nnb200_beam_select_scratch_bytes": _sz,
+    "nnb200_gpt_batch_workspace_bytes": _ll, "nnb200_paged_attention_scratch_bytes": _sz, "nnb200_beam_select_scratch_bytes": _sz,
     "nnb200_eval_expr_scratch_floats": _sz, "nnb200_rt_stream": C.c_void_p,
 }
 # functions whose int return value is a count, not a status

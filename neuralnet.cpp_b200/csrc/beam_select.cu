@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(W * 32) select_pick_kernel(const __grid_consta
 // Blocks for a row: as many as keep the machine busy where there are few rows, whole tiles each.
 static int select_spans(int groups, int beams, int vocab)
 {
-    const long long rows = static_cast<long long>(groups) * beams, tiles = ceil_div(vocab, kSelTile);
+    const long long rows = std::max(1LL, static_cast<long long>(groups) * beams), tiles = ceil_div(vocab, kSelTile);
     const long long want = std::max<long long>(1, 148 * 4 / rows), per = ceil_div(tiles, std::min(tiles, want));
     return static_cast<int>(ceil_div(tiles, per));
 }

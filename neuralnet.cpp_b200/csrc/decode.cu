@@ -494,12 +494,17 @@ static int forward_step_t(const nnb200_gpt_config& c, const float* P, const WT* 
     return gemv<WT, true, 4, 0>(Wt + L.lm_w, x, P + L.lnf_g, PB(L.lnf_b), ln, P + L.lm_b, nullptr, logits_out ? logits_out : F(W.logits), c.vocab, d, s);
 }
 
-// Y[n, out] = X[n, in] W[out, in]^T + bias (+ residual), fp32 rows times fp32 or bf16 weights
-static int prompt_linear(const float* X, const float* W, const float* bias, const float* residual, float* Y, int n, int in, int out, cudaStream_t s)
+DecodeCache decode_cache(const nnb200_gpt_config& c)
+{
+    const DecodeWs W = decode_ws(c);
+    return {W.kv, W.table};
+}
+
+int prompt_linear(const float* X, const float* W, const float* bias, const float* residual, float* Y, int n, int in, int out, cudaStream_t s)
 {
     return sgemm_strided(X, W, Y, n, out, in, in, 1, in, 1, out, 1, 0, 0, 0, 1.0f, bias, nullptr, residual, 0, s);
 }
-static int prompt_linear(const float* X, const bf16* W, const float* bias, const float* residual, float* Y, int n, int in, int out, cudaStream_t s)
+int prompt_linear(const float* X, const bf16* W, const float* bias, const float* residual, float* Y, int n, int in, int out, cudaStream_t s)
 {
     return gemm_f32_bf16(X, W, Y, n, out, in, bias, residual, s);
 }

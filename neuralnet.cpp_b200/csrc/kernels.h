@@ -13,6 +13,13 @@ struct DecodeLayer { long long wqkv, bqkv, wo, bo, g1, be1, w1, b1, w2, b2, g2, 
 struct DecodeLayout { long long tok_emb, pos_emb, lnf_g, lnf_b, lm_w, lm_b; std::vector<DecodeLayer> layers; };
 DecodeLayout decode_layout(const ::nnb200_gpt_config& c);
 
+// ---- decode.cu : where the decode workspace keeps its cache (layers x {K, V} x seq x d_model) and position table, in bytes;
+// Y[n, out] = X[n, in] W[out, in]^T + bias (+ residual), fp32 rows times fp32 or bf16 weights
+struct DecodeCache { size_t kv, table; };
+DecodeCache decode_cache(const ::nnb200_gpt_config& c);
+int prompt_linear(const float* X, const float* W, const float* bias, const float* residual, float* Y, int n, int in, int out, cudaStream_t s);
+int prompt_linear(const float* X, const bf16* W, const float* bias, const float* residual, float* Y, int n, int in, int out, cudaStream_t s);
+
 // ---- gemm_f32.cu : fp32 products on the bf16 tensor cores; each operand contiguous along one index, optional batch
 int sgemm_strided(const float* A, const float* B, float* C, int M, int N, int K, long long sam, long long sak,
                   long long sbn, long long sbk, long long ldc, int batch, long long batch_a, long long batch_b,

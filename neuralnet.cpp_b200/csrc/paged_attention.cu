@@ -1244,7 +1244,7 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     p.tc = kv.dtype == 1 && rows > 64 && kv.head_dim <= 128 && prefix_stride > 0;
     p.rt = kv.dtype == 0 ? 16 : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 128 ? 32 : 64))));
     p.own_rows = p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
-    p.row_tiles = static_cast<int>(ceil_div(rows, p.rt));
+    p.row_tiles = static_cast<int>(std::max(1LL, ceil_div(rows, p.rt)));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
     p.block_warps = !p.tc ? 4 : (kv.head_dim <= 64 ? AttnTc<64>::OWN_WARPS : AttnTc<128>::OWN_WARPS);
     const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
@@ -1254,7 +1254,7 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     long long chunk = ceil_div((p.tc ? 0 : pre_units * pre) + own_units * own, blocks);
     chunk = std::min<long long>(std::max<long long>(ceil_div(chunk, 64) * 64, 128), 1 << 20);
     p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
-    if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / pre_units, 1), ceil_div(pre, 512)));
+    if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / std::max(pre_units, 1LL), 1), ceil_div(pre, 512)));
     p.own_splits = static_cast<int>(ceil_div(own, chunk));
     p.own_warps = kv.dtype == 0 || ceil_div(own, std::max(1, p.own_splits)) > 512 ? p.block_warps : 1;
     return p;

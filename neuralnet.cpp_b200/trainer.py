@@ -403,6 +403,62 @@ class GptTrainer:
             cur_len += 1
         return generated
 
+    def generate_beam(self, prompt: Sequence[int], beams: int, max_new_tokens: int, eos_token_id: int = -1,
+                      length_penalty: float = 0.0) -> List[tuple]:
+        """Beam search: the `beams` most probable continuations kept at every token, by summed log-probability (no counterpart
+        in the reference, whose generate follows one).  The prompt is run once; its keys and values are shared by all beams,
+        each of which has pages of its own for its tokens.  Returns (tokens, score) per beam, best first by score /
+        len(tokens)**length_penalty; tokens end before eos_token_id (-1: there is none), whose probability counts.  The prompt and
+        the new tokens must fit into seq; 1 <= beams <= 64."""
+        n, new, vocab = len(prompt), int(max_new_tokens), self.cfg.vocab
+        if not (n >= 1 and new >= 1 and n + new <= self.cfg.seq):
+            raise ValueError("prompt and new tokens must be there and fit into seq")
+        if not 1 <= beams <= min(64, vocab):
+            raise ValueError("1 to 64 beams, and no more than the vocabulary has tokens")
+        if not -1 <= eos_token_id < vocab:
+            raise ValueError("eos_token_id must be in the vocabulary, or -1")
+        i32 = dict(dtype=torch.int32, device=self.device)
+        first = self.prefill(prompt)
+        dec, _ = self._decode_state()
+        size = int(call("nnb200_gpt_batch_workspace_bytes", C.byref(self._c), beams, new))
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        scratch = torch.empty(max(call("nnb200_beam_select_scratch_bytes", 1, b, vocab, beams) for b in (1, beams)), dtype=torch.uint8, device=self.device)
+        logits = torch.empty((beams, vocab), dtype=torch.float32, device=self.device)
+        # a row per token: the beam it continues, the token, the score so far, whether it has ended; one row in front for the prompt
+        parent, token, ended = (torch.zeros((new + 1, beams), **i32) for _ in range(3))
+        score = torch.zeros((new + 1, beams), dtype=torch.float32, device=self.device)
+        call("nnb200_gpt_batch_begin", C.byref(self._c), _ptr(dec), _ptr(ws), beams, new, n, _stream())
+        steps = 0
+        for step in range(new):
+            at, to = step, step + 1
+            call("nnb200_beam_select", _ptr(logits if step else first), vocab, 0, 1, beams if step else 1, vocab, _ptr(score[at]),
+                 _ptr(ended[at]) if eos_token_id >= 0 else None, eos_token_id, beams, _ptr(parent[to]), _ptr(token[to]), _ptr(score[to]), _ptr(ended[to]),
+                 _ptr(scratch), scratch.numel(), _stream())
+            steps = to
+            if to == new or (eos_token_id >= 0 and bool(ended[to].all())):
+                break
+            if step:
+                call("nnb200_gpt_batch_reorder", C.byref(self._c), _ptr(ws), beams, new, _ptr(parent[to]), _stream())
+            call("nnb200_gpt_batch_step", C.byref(self._c), _ptr(self.params), _ptr(self.shadow), _ptr(dec), _ptr(ws), beams, new, n, step, _ptr(token[to]),
+                 _ptr(logits), _stream())
+        parent, token, score = parent.cpu().numpy(), token.cpu().numpy(), score[steps].cpu().numpy()
+        found = []
+        for b in range(beams):
+            tokens, at = [], b
+            for s in range(steps, 0, -1):
+                if parent[s, at] < 0:                    # nothing was left for this beam: NaN logits
+                    tokens = None
+                    break
+                tokens.append(int(token[s, at]))
+                at = int(parent[s, at])
+            if tokens is None:
+                continue
+            tokens.reverse()
+            if eos_token_id in tokens:
+                tokens = tokens[:tokens.index(eos_token_id)]
+            found.append((tokens, float(score[b])))
+        return sorted(found, key=lambda f: -f[1] / max(1, len(f[0])) ** length_penalty)
+
     def loss_tensor(self) -> torch.Tensor:
         """Device view of the scalar loss of the last loss_and_grad call."""
         o = self._off["loss"]

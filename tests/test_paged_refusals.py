@@ -103,5 +103,41 @@ def test_empty_calls_do_nothing():
     assert nnb.lib.nnb200_beam_reorder(*reorder_args(beams=0)) == 0
 
 
+def test_scratch_of_empty_calls():
+    for groups, size in ((0, 0), (0, 100), (3, 0)):
+        assert nnb.lib.nnb200_paged_attention_scratch_bytes(C.byref(kv()), groups, size, 4, 4, 2) < 1024
+    assert nnb.lib.nnb200_beam_select_scratch_bytes(0, 4, 100, 8) < 1024
+
+
 def test_one_layer_needs_no_stride():
     assert nnb.lib.nnb200_paged_append(*append_args(kv(layers=1, layer_stride=0), tokens=0)) == 0
+
+
+def batch_cfg(**change):
+    a = dict(vocab=72, d_model=128, heads=2, layers=2, d_ff=104, seq=64, batch=1, act=1, norm=1, pos=3, precision=0)
+    a.update(change)
+    return nnb.GptConfig(*a.values()).c_struct()
+
+
+@pytest.mark.parametrize("change,seqs,rows", [({}, 0, 4), ({}, 1025, 4), ({}, 4, 0), ({}, 4, 65), (dict(d_model=24, heads=2), 4, 4), (dict(d_model=528, heads=2), 4, 4),
+                                              (dict(d_model=130), 4, 4), (dict(seq=1 << 22), 1024, 1 << 22)])
+def test_batch_refuses_shapes(change, seqs, rows):
+    c = batch_cfg(**change)
+    assert nnb.lib.nnb200_gpt_batch_workspace_bytes(C.byref(c), seqs, rows) == -1
+    refused("nnb200_gpt_batch_begin", C.byref(c), P, P, seqs, rows, 10, None)
+    refused("nnb200_gpt_batch_step", C.byref(c), P, P, P, P, seqs, rows, 10, 0, P, P, None)
+    refused("nnb200_gpt_batch_reorder", C.byref(c), P, seqs, rows, P, None)
+
+
+def test_batch_refuses_arguments():
+    c = batch_cfg()
+    assert nnb.lib.nnb200_gpt_batch_workspace_bytes(C.byref(c), 4, 8) > 0
+    for args in ((None, P, 4, 8, 10), (P, None, 4, 8, 10), (P, P + 128, 4, 8, 10), (P, P, 4, 8, 0), (P, P, 4, 8, 57), (P, P, 4, 8, -1)):
+        refused("nnb200_gpt_batch_begin", C.byref(c), *args, None)
+    good = dict(params=P, bf16=None, dec=P, ws=P, seqs=4, rows=8, prompt=10, step=0, tokens=P, logits=P)
+    for change in (dict(params=None), dict(dec=None), dict(ws=None), dict(tokens=None), dict(logits=None), dict(params=P + 8), dict(ws=P + 16), dict(logits=P + 4), dict(step=-1),
+                   dict(step=8), dict(prompt=0), dict(prompt=57)):
+        refused("nnb200_gpt_batch_step", C.byref(c), *{**good, **change}.values(), None)
+    refused("nnb200_gpt_batch_step", C.byref(batch_cfg(precision=1)), *good.values(), None)
+    refused("nnb200_gpt_batch_reorder", C.byref(c), None, 4, 8, P, None)
+    refused("nnb200_gpt_batch_reorder", C.byref(c), P, 4, 8, None, None)
