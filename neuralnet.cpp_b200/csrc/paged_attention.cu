@@ -12,6 +12,7 @@
 #include "tc_ptx.cuh"
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 namespace nnb {
@@ -30,6 +31,7 @@ struct PagedAttnArgs {
     int slots, pre_slots, own_rows; // places of a query row's partial results, the prefix's among them; rows of an own tile
     int own_warps;                  // warps that share a task of own rows: all of a block, or 1 (a task for each)
     int pre_blocks, tasks;          // tasks [0, pre_blocks) are prefixes, a block each; the others own rows
+    int direct;                     // a block takes a sequence's prefix and its own rows
     int pairs, vectors;             // queries may be read two columns, or 16 bytes, at a time
     float c;                        // log2(e) / sqrt(head_dim): exponentials are powers of two
     float* part;                    // (query row, slot): head_dim sums
@@ -47,8 +49,8 @@ __device__ __forceinline__ float alibi_slope2(int h, int heads) { return exp2f(-
 // What a block works on: `rows` query rows (row r is query head head0 + r % m of sequence seq0 + r / m) against rows
 // [begin, end) of one page table.  Row t stands at position place + t of what sequence `seq` sees in all.
 struct AttnTask {
-    const int* table;
-    int hk, first, rows, begin, end, place, slot, group;
+    const int *table, *table2;
+    int hk, first, rows, begin, end, place, slot, group, end2;  // end2: rows of a second run, behind the first (short contexts, fp32)
 };
 // lengths are device data: clamped to [0, what the table holds]; negative own length: nothing is seen
 __device__ __forceinline__ int held(int len, int stride, int shift)
@@ -66,6 +68,8 @@ template <int RT, typename T>
 __device__ __forceinline__ AttnTask task_of(const PagedPool<T>& pool, const PagedAttnArgs& a, int b)
 {
     AttnTask k;
+    k.table2 = nullptr;
+    k.end2 = 0;
     if (b < a.pre_blocks) {                                     // neighbours share their cached rows: row tiles, then splits
         int rest = a.row_tiles.split(b);                        // b: row tile
         int head = a.pre_splits.split(rest);                    // rest: split
@@ -90,6 +94,16 @@ __device__ __forceinline__ AttnTask task_of(const PagedPool<T>& pool, const Page
     k.table = a.table + static_cast<long long>(seq) * a.table_stride;
     k.place = a.prefix_stride ? held(a.prefix_len[k.group], a.prefix_stride, pool.page_shift) : 0;
     k.slot = a.pre_slots + rest;
+    if (a.direct) {                                             // the prefix, then the sequence's own rows, by one block
+        k.table2 = k.table;
+        k.table = a.prefix_table + static_cast<long long>(k.group) * a.prefix_stride;
+        k.begin = 0;
+        k.end = a.len[seq] < 0 ? 0 : k.place;
+        k.end2 = a.table_stride ? held(a.len[seq], a.table_stride, pool.page_shift) : 0;
+        k.place = 0;
+        k.slot = 0;
+        return k;
+    }
     share_of(held(a.len[seq], a.table_stride, pool.page_shift), static_cast<int>(a.own_splits.d), rest, k.begin, k.end);
     return k;
 }
@@ -105,7 +119,7 @@ __device__ __forceinline__ AttnRow row_of(const PagedAttnArgs& a, const AttnTask
 __device__ __forceinline__ int far_of(const PagedAttnArgs& a, int shift, const AttnTask& k, int seq)
 {
     const int pre = a.prefix_stride ? held(a.prefix_len[k.group], a.prefix_stride, shift) : 0;
-    return pre + (a.table_stride ? held(a.len[seq], a.table_stride, shift) : 0) - 1 - k.place;
+    return pre + (a.table_stride ? held(a.len[seq], a.table_stride, shift) : 0) - 1 - k.place;   // place is 0 where a task has both runs
 }
 
 // ---------------------------------------------------------------- bf16: mma.sync tiles
@@ -395,13 +409,15 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
     using Str = AttnStream<DP>;
     constexpr int KW = Str::KW, NK = KW / 16, ND = DP / 16, KS = DP / 16, ST = Str::ST, CPR = Str::CPR;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wk = wt == 1 ? 0 : warp, dk = pool.dk;
-    const int all = (k.end - k.begin + KW - 1) / KW, steps = (all - wk + wt - 1) / wt;
+    const int run1 = (k.end - k.begin + KW - 1) / KW, all = run1 + (k.end2 + KW - 1) / KW, steps = (all - wk + wt - 1) / wt;
     const uint32_t ring = smem_u32(smem) + warp * Str::RING;
     uint32_t* alive = reinterpret_cast<uint32_t*>(smem + NW * Str::RING) + warp * 4;
     // the cached row this lane looks up for a step (lanes beyond KW: none)
     auto look = [&](int step) {
-        const int t = k.begin + (step * wt + wk) * KW + lane;
-        return step < steps && lane < KW && t < k.end ? pool.find(k.table, k.hk, t) : -1;
+        const int at = step * wt + wk;
+        const bool second = at >= run1;                         // short contexts: the sequence's own rows behind the prefix
+        const int t = second ? (at - run1) * KW + lane : k.begin + at * KW + lane;
+        return step < steps && lane < KW && t < (second ? k.end2 : k.end) ? pool.find(second ? k.table2 : k.table, k.hk, t) : -1;
     };
     // lane l copies chunk l % CPR of rows l / CPR, l / CPR + RPI, ..
     constexpr int RPI = 32 / CPR;                               // rows the warp copies at once
@@ -495,7 +511,8 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
             }
         }
         if (a.alibi) {
-            const float t0 = static_cast<float>(k.begin + (step * wt + wk) * KW + g);
+            const int at = step * wt + wk;
+            const float t0 = static_cast<float>((at >= run1 ? k.end + (at - run1) * KW : k.begin + at * KW) + g);
 #pragma unroll
             for (int x = 0; x < NK; ++x)
 #pragma unroll
@@ -628,7 +645,7 @@ __device__ __forceinline__ void own_bf16(const PagedPool<bf16>& pool, const Page
     const int task = a.pre_blocks + (shared ? b : b * NW + static_cast<int>(threadIdx.x >> 5));
     if (task >= a.tasks) return;
     const AttnTask k = task_of<RT>(pool, a, task);
-    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, shared ? threadIdx.x : threadIdx.x & 31, shared ? 32 * NW : 32); return; }
+    if (k.begin >= k.end && k.end2 == 0) { leave_nothing<bf16>(a, k, pool.dk, shared ? threadIdx.x : threadIdx.x & 31, shared ? 32 * NW : 32); return; }
     stream_bf16<DP, NQ, NW>(pool, a, k, smem, a.own_warps);
 }
 
@@ -1014,76 +1031,70 @@ int paged_attn_device_error(int* code)
 }
 
 // ---------------------------------------------------------------- fp32: FMA tiles
-// Up to 16 query rows against KT cached rows a step.  Scores: a thread takes one cached row and four to eight query rows; softmax:
-// eight lanes a query row; values: a thread takes four columns and every KG-th cached row, for all query rows, and the KG
-// parts are summed at the end.  Rows in shared memory are 16 bytes longer than they are, so that eight neighbours' 16-byte reads
-// meet no bank twice.  fp32 products and sums throughout: infinities and NaN behave as in the formula, which splitting a
-// number into parts for the tensor cores would not keep.
-template <int DP> struct AttnTile32 {
+// RT (4, 8 or 16) query rows against KT cached rows a step, 256 threads.  Scores: a thread takes one cached row and RT KT / 256 query
+// rows; softmax: up to a warp per query row; values: a thread takes four columns and every KG-th cached row, for all query rows,
+// and the KG parts are summed at the end.  Rows in shared memory are 16 bytes longer than they are, so that eight neighbours'
+// 16-byte reads meet no bank twice.  fp32 products and sums throughout: infinities and NaN behave as in the formula, which
+// splitting a number into parts for the tensor cores would not keep.  With few rows a step is a chain of dependent
+// instructions: eight warps and a fixed RT, instead of four that count rows, took 13.5 us to 10.9 for eight beams of 12 heads
+// behind 901 rows.
+constexpr int kF32Threads = 256;
+template <int DP, int RT> struct AttnTile32 {
     static constexpr int KT = DP <= 64 ? 64 : 4096 / DP, LD = DP + 4, CPR = DP / 4, STAGES = 2;
-    static constexpr int G = 128 / KT, RPT = 16 / G;           // sets of query rows, rows of a thread
-    static constexpr int KG = 512 / DP, PL = 20;               // sets of cached rows for the values, row of the weights
+    static constexpr int SETS = kF32Threads / KT, RPT = RT > SETS ? RT / SETS : 1;      // sets of threads, query rows of each
+    static constexpr int KG = kF32Threads * 4 / DP, PL = RT + 4;   // sets of cached rows for the values, row of the weights
+    static constexpr int LPR = kF32Threads / RT < 32 ? kF32Threads / RT : 32, KPL = KT / LPR > 0 ? KT / LPR : 1;   // lanes of a softmax row, cached rows of each
     static constexpr int FLOATS = KT * LD;                     // K, or V, of a stage
-    static constexpr int RING = STAGES * 2 * FLOATS;
-    static constexpr int SMEM = (RING + 16 * DP + KT * PL + 16 * 4) * 4 + STAGES * (KT + 16);
-    static_assert(RING >= 128 * 64, "the join fits the ring");
-    // query row i of set g: fours of rows in turn, so that few rows still spread over the sets
-    static __device__ __forceinline__ int row(int g, int i) { return RPT >= 4 ? (i >> 2) * 4 * G + g * 4 + (i & 3) : g * RPT + i; }
+    static constexpr int RING = STAGES * 2 * FLOATS > KG * RT * DP ? STAGES * 2 * FLOATS : KG * RT * DP;
+    static constexpr int SMEM = (RING + RT * DP + KT * PL + 4 * RT) * 4 + STAGES * KT;
 };
 
-template <int DP>
-__device__ __forceinline__ void load_f32(const PagedPool<float>& pool, const AttnTask& k, uint32_t base, uint8_t* alive, int step, int stage)
+template <int DP, int RT>
+__device__ __forceinline__ void attend_f32(const PagedPool<float>& pool, const PagedAttnArgs& a, const AttnTask& k, uint8_t* smem)
 {
-    using Tile = AttnTile32<DP>;
-    const int t0 = k.begin + step * Tile::KT, tid = threadIdx.x;
-#pragma unroll
-    for (int i = 0; i < Tile::KT * Tile::CPR / 128; ++i) {
-        const int idx = tid + i * 128, r = idx / Tile::CPR, c = idx % Tile::CPR, t = t0 + r;
-        const int row = t < k.end ? pool.find(k.table, k.hk, t) : -1;
-        const bool there = row >= 0;
-        const long long off = there && c * 4 < pool.dk ? static_cast<long long>(row) * pool.dk + c * 4 : 0;
-        const int bytes = there && c * 4 < pool.dk ? 16 : 0;
-        const uint32_t dst = base + (stage * 2 * Tile::FLOATS + r * Tile::LD + c * 4) * 4;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pool.k + off), "r"(bytes) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Tile::FLOATS * 4), "l"(pool.v + off), "r"(bytes) : "memory");
-        if (c == 0) alive[stage * (Tile::KT + 16) + r] = there;
-    }
-}
-
-template <int DP>
-__global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> pool, const __grid_constant__ PagedAttnArgs a)
-{
-    extern __shared__ __align__(1024) uint8_t smem[];
-    using Tile = AttnTile32<DP>;
-    constexpr int KT = Tile::KT, ST = Tile::STAGES, PL = Tile::PL;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const AttnTask k = task_of<16>(pool, a, blockIdx.x);
-    if (k.begin >= k.end) { leave_nothing<float>(a, k, pool.dk, threadIdx.x, 128); return; }
-    const int tid = threadIdx.x, dk = pool.dk, steps = (k.end - k.begin + KT - 1) / KT;
+    using Tile = AttnTile32<DP, RT>;
+    constexpr int KT = Tile::KT, ST = Tile::STAGES, PL = Tile::PL, NTH = kF32Threads;
+    const int tid = threadIdx.x, dk = pool.dk, steps1 = max(0, (k.end - k.begin + KT - 1) / KT), steps = steps1 + (k.end2 + KT - 1) / KT;
+    if (steps == 0) { leave_nothing<float>(a, k, dk, tid, NTH); return; }
     float* ring = reinterpret_cast<float*>(smem);
-    float *sq = ring + Tile::RING, *sp = sq + 16 * DP, *sback = sp + KT * PL, *sslope = sback + 16, *sfar = sslope + 16;
-    uint8_t* alive = reinterpret_cast<uint8_t*>(sfar + 32);
+    float *sq = ring + Tile::RING, *sp = sq + RT * DP, *sback = sp + KT * PL, *sslope = sback + RT, *sfar = sslope + RT;
+    uint8_t* alive = reinterpret_cast<uint8_t*>(sfar + 2 * RT);
     const uint32_t base = smem_u32(ring);
+    auto load = [&](int step, int stage) {
+        const bool second = step >= steps1;
+        const int* table = second ? k.table2 : k.table;
+        const int t0 = second ? (step - steps1) * KT : k.begin + step * KT, end = second ? k.end2 : k.end;
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) { if (i < steps) load_f32<DP>(pool, k, base, alive, i, i); cp_commit(); }
-    for (int i = tid; i < 16 * DP; i += 128) {
+        for (int i = 0; i < KT * Tile::CPR / NTH; ++i) {
+            const int idx = tid + i * NTH, r = idx / Tile::CPR, c = idx % Tile::CPR, t = t0 + r;
+            const int row = t < end ? pool.find(table, k.hk, t) : -1;
+            const bool there = row >= 0, in = there && c * 4 < dk;
+            const long long off = in ? static_cast<long long>(row) * dk + c * 4 : 0;
+            const uint32_t dst = base + (stage * 2 * Tile::FLOATS + r * Tile::LD + c * 4) * 4;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(pool.k + off), "r"(in ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Tile::FLOATS * 4), "l"(pool.v + off), "r"(in ? 16 : 0) : "memory");
+            if (c == 0) alive[stage * KT + r] = there;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) { if (i < steps) load(i, i); cp_commit(); }
+    for (int i = tid; i < RT * DP; i += NTH) {
         const int r = i / DP, c = i - r * DP;
-        const AttnRow w = row_of(a, k, r);
+        const AttnRow w = row_of(a, k, min(r, k.rows - 1));
         sq[i] = r < k.rows && c < dk ? static_cast<const float*>(a.q)[w.seq * a.ldq + static_cast<long long>(w.head) * dk + c] : 0.f;
     }
-    if (tid < 16) {
+    if (tid < RT) {
         const bool on = a.alibi && tid < k.rows;
         const AttnRow w = row_of(a, k, on ? tid : 0);
         sslope[tid] = on ? alibi_slope2(w.head, a.heads) : 0.f;
         sfar[tid] = on ? static_cast<float>(far_of(a, pool.page_shift, k, w.seq)) : 0.f;
     }
-    const int key = tid % KT, set = tid / KT;                   // scores
-    const int srow = tid >> 3, part = tid & 7;                  // softmax
+    const int key = tid % KT, set = tid / KT;                   // scores: query rows set, set + SETS, ..
+    const int srow = tid / Tile::LPR, part = tid % Tile::LPR;   // softmax
     const int c4 = tid % (DP / 4), kg = tid / (DP / 4);         // values
-    const int quads = (k.rows + 3) >> 2;
-    float m = -INFINITY, l = 0.f, o[16][4];
+    float m = -INFINITY, l = 0.f, o[RT][4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[r][j] = 0.f;
 
@@ -1091,10 +1102,10 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
         cp_wait<ST - 2>();
         __syncthreads();
         const int stage = step % ST;
-        if (step + ST - 1 < steps) load_f32<DP>(pool, k, base, alive, step + ST - 1, (step + ST - 1) % ST);
+        if (step + ST - 1 < steps) load(step + ST - 1, (step + ST - 1) % ST);
         cp_commit();
         const float *sk = ring + stage * 2 * Tile::FLOATS, *sv = sk + Tile::FLOATS;
-        {
+        if (set < RT) {
             float s[Tile::RPT];
 #pragma unroll
             for (int i = 0; i < Tile::RPT; ++i) s[i] = 0.f;
@@ -1103,46 +1114,41 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
                 const float4 kv = *reinterpret_cast<const float4*>(sk + key * Tile::LD + d);
 #pragma unroll
                 for (int i = 0; i < Tile::RPT; ++i) {
-                    if (Tile::row(set, i) >= k.rows) continue;
-                    const float4 q = *reinterpret_cast<const float4*>(sq + Tile::row(set, i) * DP + d);
+                    const float4 q = *reinterpret_cast<const float4*>(sq + (set + Tile::SETS * i) * DP + d);
                     s[i] = fmaf(q.x, kv.x, s[i]); s[i] = fmaf(q.y, kv.y, s[i]); s[i] = fmaf(q.z, kv.z, s[i]); s[i] = fmaf(q.w, kv.w, s[i]);
                 }
             }
-            const bool there = alive[stage * (KT + 16) + key];
-            const float t = static_cast<float>(k.begin + step * KT + key);
+            const bool there = alive[stage * KT + key];
+            const float t = static_cast<float>((step >= steps1 ? k.end + (step - steps1) * KT : k.begin + step * KT) + key);
 #pragma unroll
             for (int i = 0; i < Tile::RPT; ++i) {
-                const int r = Tile::row(set, i);
-                s[i] = there ? s[i] * a.c - sslope[r] * (sfar[r] - t) : -INFINITY;
-            }
-            if constexpr (Tile::RPT >= 4) {
-#pragma unroll
-                for (int i = 0; i < Tile::RPT; i += 4) *reinterpret_cast<float4*>(sp + key * PL + Tile::row(set, i)) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < Tile::RPT; ++i) sp[key * PL + Tile::row(set, i)] = s[i];
+                const int r = set + Tile::SETS * i;
+                sp[key * PL + r] = there ? s[i] * a.c - sslope[r] * (sfar[r] - t) : -INFINITY;
             }
         }
         __syncthreads();
-        float s[KT / 8], top = m;
+        bool moved = false;
+        if (srow < RT) {
+            float s[Tile::KPL], top = m;
 #pragma unroll
-        for (int j = 0; j < KT / 8; ++j) { s[j] = sp[(part + 8 * j) * PL + srow]; top = fmaxf(top, s[j]); }
+            for (int j = 0; j < Tile::KPL; ++j) { s[j] = part + Tile::LPR * j < KT ? sp[(part + Tile::LPR * j) * PL + srow] : -INFINITY; top = fmaxf(top, s[j]); }
 #pragma unroll
-        for (int w = 1; w < 8; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        const float ref = top == -INFINITY ? 0.f : top, back = exp2f(m - ref);
-        const bool moved = top != m;
-        l *= back;
-        m = top;
+            for (int w = 1; w < Tile::LPR; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float ref = top == -INFINITY ? 0.f : top, back = exp2f(m - ref);
+            moved = top != m;
+            l *= back;
+            m = top;
 #pragma unroll
-        for (int j = 0; j < KT / 8; ++j) {
-            s[j] = exp2f(s[j] - ref);
-            l += s[j];
-            sp[(part + 8 * j) * PL + srow] = s[j];
+            for (int j = 0; j < Tile::KPL; ++j) {
+                s[j] = exp2f(s[j] - ref);
+                l += s[j];
+                if (part + Tile::LPR * j < KT) sp[(part + Tile::LPR * j) * PL + srow] = s[j];
+            }
+            if (part == 0) sback[srow] = back;
         }
-        if (part == 0) sback[srow] = back;
         if (__syncthreads_or(moved)) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < RT; ++r) {
                 const float b = sback[r];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[r][j] *= b;
@@ -1152,8 +1158,7 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
         for (int t = kg; t < KT; t += Tile::KG) {
             const float4 v = *reinterpret_cast<const float4*>(sv + t * Tile::LD + c4 * 4);
 #pragma unroll
-            for (int rq = 0; rq < 4; ++rq) {
-                if (rq >= quads) break;
+            for (int rq = 0; rq < RT / 4; ++rq) {
                 const float4 p = *reinterpret_cast<const float4*>(sp + t * PL + rq * 4);
                 const float pr[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
@@ -1165,25 +1170,37 @@ __global__ void __launch_bounds__(128) paged_attn_f32_kernel(PagedPool<float> po
         }
     }
 #pragma unroll
-    for (int w = 1; w < 8; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    for (int w = 1; w < Tile::LPR; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
     cp_wait<0>();
     __syncthreads();
-    if (part == 0) { sslope[srow] = m; sfar[srow] = l; }
+    if (part == 0 && srow < RT) { sslope[srow] = m; sfar[srow] = l; }
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-        if (r < k.rows) *reinterpret_cast<float4*>(ring + (kg * 16 + r) * DP + c4 * 4) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+    for (int r = 0; r < RT; ++r)
+        if (r < k.rows) *reinterpret_cast<float4*>(ring + (kg * RT + r) * DP + c4 * 4) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
     __syncthreads();
     const int vecs = dk / 4;
-    for (int idx = tid; idx < k.rows * vecs; idx += 128) {
+    for (int idx = tid; idx < k.rows * vecs; idx += NTH) {
         const int r = a.by_vecs.div(idx), c = (idx - r * vecs) * 4;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < Tile::KG; ++w) {
-            const float4 y = *reinterpret_cast<const float4*>(ring + (w * 16 + r) * DP + c);
+            const float4 y = *reinterpret_cast<const float4*>(ring + (w * RT + r) * DP + c);
             x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         leave<float>(a, k, dk, r, c, x, sslope[r], sfar[r]);
     }
+}
+
+// RT rows of a group against its prefix, RO of a sequence against its own rows
+template <int DP, int RT, int RO>
+__global__ void __launch_bounds__(kF32Threads) paged_attn_f32_kernel(PagedPool<float> pool, const __grid_constant__ PagedAttnArgs a)
+{
+    extern __shared__ __align__(1024) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int b = static_cast<int>(blockIdx.x);
+    const AttnTask k = task_of<RT>(pool, a, b);
+    if (RT == RO || b < a.pre_blocks) attend_f32<DP, RT>(pool, a, k, smem);
+    else attend_f32<DP, RO>(pool, a, k, smem);
 }
 
 // ---------------------------------------------------------------- the join
@@ -1233,7 +1250,7 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------- how the work is cut
-struct AttnPlan { bool tc; int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps, block_warps; };
+struct AttnPlan { bool tc, direct; int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps, block_warps; };
 static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int heads, int prefix_stride, int table_stride)
 {
     AttnPlan p;
@@ -1242,8 +1259,9 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     // fp32 tiles take 16 query rows; bf16 streams 8 or 16; beyond that tcgen05 tiles take 128, and where a head is too wide
     // for those mma.sync tiles take 64
     p.tc = kv.dtype == 1 && rows > 64 && kv.head_dim <= 128 && prefix_stride > 0;
-    p.rt = kv.dtype == 0 ? 16 : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 128 ? 32 : 64))));
-    p.own_rows = p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
+    const int few = std::max<long long>(prefix_stride > 0 ? rows : 0, m) <= 4 ? 4 : (std::max<long long>(prefix_stride > 0 ? rows : 0, m) <= 8 ? 8 : 16);
+    p.rt = kv.dtype == 0 ? few : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 128 ? 32 : 64))));
+    p.own_rows = kv.dtype == 0 ? (m <= 4 ? 4 : p.rt) : p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
     p.row_tiles = static_cast<int>(std::max(1LL, ceil_div(rows, p.rt)));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
     p.block_warps = !p.tc ? 4 : (kv.head_dim <= 64 ? AttnTc<64>::OWN_WARPS : AttnTc<128>::OWN_WARPS);
@@ -1256,7 +1274,17 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
     if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / std::max(pre_units, 1LL), 1), ceil_div(pre, 512)));
     p.own_splits = static_cast<int>(ceil_div(own, chunk));
-    p.own_warps = kv.dtype == 0 || ceil_div(own, std::max(1, p.own_splits)) > 512 ? p.block_warps : 1;
+    if (getenv("OC")) { long long oc = std::max(64LL, std::min(chunk, ceil_div(ceil_div(own_units * own, 148LL * 16 * atoi(getenv("OC"))), 64) * 64)); p.own_splits = static_cast<int>(ceil_div(own, oc)); }
+    // a prefix and own rows of 128 at most: a block for both, without the join, takes 5.4 us where prefix, own rows and join take 7.6
+    // (four beams of six heads behind 41 rows; behind 200 it would be 10.5 and 7.9)
+    p.direct = !p.tc && pre > 0 && own > 0 && pre + own <= 128 && static_cast<long long>(groups) * size * kv.kv_heads <= 4 * 148;
+    if (p.direct) {
+        p.rt = p.own_rows = kv.dtype == 0 && m <= 4 ? 4 : (m <= 8 ? 8 : 16);
+        p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
+        p.pre_splits = 0;
+        p.own_splits = 1;
+    }
+    p.own_warps = kv.dtype == 0 || p.direct || ceil_div(own, std::max(1, p.own_splits)) > 512 ? p.block_warps : 1;
     return p;
 }
 
@@ -1268,7 +1296,7 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
     a.m = FastDiv(a.heads / kv.kv_heads);
     a.row_tiles = FastDiv(p.row_tiles); a.own_tiles = FastDiv(p.own_tiles); a.pre_splits = FastDiv(p.pre_splits); a.own_splits = FastDiv(p.own_splits);
     a.by_size = FastDiv(a.size); a.by_kv_heads = FastDiv(kv.kv_heads); a.by_vecs = FastDiv(kv.head_dim / 4); a.by_heads = FastDiv(a.heads);
-    a.pre_slots = p.pre_splits; a.slots = p.pre_splits + p.own_splits; a.own_rows = p.own_rows; a.own_warps = p.own_warps;
+    a.pre_slots = p.pre_splits; a.slots = p.pre_splits + p.own_splits; a.own_rows = p.own_rows; a.own_warps = p.own_warps; a.direct = p.direct ? 1 : 0;
     const long long pre_tasks = static_cast<long long>(a.groups) * kv.kv_heads * p.row_tiles * p.pre_splits;
     const long long own_tasks = static_cast<long long>(a.groups) * a.size * kv.kv_heads * p.own_tiles * p.own_splits;
     NNB_ARG_CHECK(pre_tasks + own_tasks <= INT_MAX, "too many queries for one call");
@@ -1283,14 +1311,19 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
     if (blocks > 0) {
         auto go = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
             NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
-            kernel<<<static_cast<unsigned>(blocks), 128, bytes, s>>>(pool, a);
+            kernel<<<static_cast<unsigned>(blocks), sizeof(T) == 4 ? kF32Threads : 128, bytes, s>>>(pool, a);
             NNB_LAUNCH_CHECK();
             return 0;
         };
         auto width = [&](auto dp) {
             constexpr int DP = decltype(dp)::value;
             static PerDeviceOnce once[6];
-            if constexpr (sizeof(T) == 4) return go(paged_attn_f32_kernel<DP>, AttnTile32<DP>::SMEM, once[0]);
+            if constexpr (sizeof(T) == 4) {
+                const bool narrow = p.own_rows == 4;
+                if (p.rt == 4) return go(paged_attn_f32_kernel<DP, 4, 4>, AttnTile32<DP, 4>::SMEM, once[0]);
+                if (p.rt == 8) return narrow ? go(paged_attn_f32_kernel<DP, 8, 4>, AttnTile32<DP, 8>::SMEM, once[1]) : go(paged_attn_f32_kernel<DP, 8, 8>, AttnTile32<DP, 8>::SMEM, once[2]);
+                return narrow ? go(paged_attn_f32_kernel<DP, 16, 4>, AttnTile32<DP, 16>::SMEM, once[3]) : go(paged_attn_f32_kernel<DP, 16, 16>, AttnTile32<DP, 16>::SMEM, once[4]);
+            }
             else {
                 const bool wide = p.own_rows == 16;
                 constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));

@@ -245,6 +245,20 @@ def test_attention_of_nothing(g, dtype):
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("heads,hk,dk,page", [(6, 6, 64, 16), (8, 2, 128, 8), (3, 1, 40, 32), (40, 2, 32, 16), (2, 2, 256, 8)])
+@pytest.mark.parametrize("alibi", [0, 1])
+def test_attention_short_contexts(g, dtype, heads, hk, dk, page, alibi):
+    """Prefix and own rows of a few steps together: lengths of nothing and one, padded sequences, both runs ending inside a step."""
+    _check_attention(g, dtype, heads, hk, dk, page, 3, 4, [41, 0, 1], [1, 17, -1, 24, 0, 1, 16, -1, 5, 0, 23, 2], alibi)
+    _check_attention(g, dtype, heads, hk, dk, page, 1, 2, [64], [64, 33], alibi, seed=1)
+
+    def change(q, kp, vp, ptab, otab, plen, olen):
+        ptab[0, 0], otab[1, 0] = -1, kp.shape[0]
+        return q, kp, vp, ptab, otab, plen, olen
+    _check_attention(g, dtype, heads, hk, dk, page, 1, 2, [40], [9, 30], alibi, seed=2, change=change)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
 def test_attention_large_scores(g, dtype):
     """Scores of hundreds: weights of almost nothing and almost everything, maxima that move from tile to tile."""
     _check_attention(g, dtype, 4, 4, 64, 16, 1, 5, [700], [50, 1, 0, 300, 7], seed=9, spread=60.0)
