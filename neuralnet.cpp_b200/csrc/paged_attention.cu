@@ -12,7 +12,6 @@
 #include "tc_ptx.cuh"
 
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 namespace nnb {
@@ -31,6 +30,7 @@ struct PagedAttnArgs {
     int slots, pre_slots, own_rows; // places of a query row's partial results, the prefix's among them; rows of an own tile
     int own_warps;                  // warps that share a task of own rows: all of a block, or 1 (a task for each)
     int pre_blocks, tasks;          // tasks [0, pre_blocks) are prefixes, a block each; the others own rows
+    int first_block;                // of this launch: the prefixes may be another's
     int direct;                     // a block takes a sequence's prefix and its own rows
     int pairs, vectors;             // queries may be read two columns, or 16 bytes, at a time
     float c;                        // log2(e) / sqrt(head_dim): exponentials are powers of two
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
     extern __shared__ __align__(1024) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int RT = WM == 1 ? NQ * 8 : WM * 16;
-    const int b = static_cast<int>(blockIdx.x);
+    const int b = static_cast<int>(blockIdx.x) + a.first_block;
     if (b >= a.pre_blocks) { own_bf16<DP, NQ, 4, RT>(pool, a, b - a.pre_blocks, smem); return; }
     const AttnTask k = task_of<RT>(pool, a, b);
     if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 128); return; }
@@ -686,8 +686,6 @@ template <int DP> struct AttnTc {
     static constexpr int TILE = NS * SUB;
     static constexpr int OFF_K = TILE, OFF_V = OFF_K + ST * TILE, OFF_P = OFF_V + ST * TILE, OFF_X = OFF_P + SUB, OFF_BAR = OFF_X + 2 * 128 * 2;
     static constexpr int TILES = OFF_BAR + 256;                 // DP = 128: two blocks fit an SM, with 256 bytes to spare
-    static constexpr int WARPS = 10, OWN_WARPS = DP == 64 ? 8 : 6;   // warps, and those that stream own rows
-    static constexpr int SMEM = TILES > AttnStream<DP>::smem(OWN_WARPS) ? TILES : AttnStream<DP>::smem(OWN_WARPS);
     static constexpr uint32_t TMEM_COLS = 256;                  // scores [0, 128), O [128, 128 + DP)
 };
 
@@ -1006,21 +1004,19 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     }
 }
 
-// Prefix blocks, bound by the tensor cores and exponentials, first; blocks of own rows, bound by memory, as they end.
+// Prefixes only.  The own rows' kernel goes first, 16 warps an SM as it needs them for memory's sake; this one's blocks move in as
+// its last ones leave.
 template <int DP>
 __global__ void __launch_bounds__(320, 2) paged_attn_tc_kernel(PagedPool<bf16> pool, const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap tk,
                                                                const __grid_constant__ CUtensorMap tv)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int b = static_cast<int>(blockIdx.x);
-    if (b >= a.pre_blocks) {
-        if (threadIdx.x < AttnTc<DP>::OWN_WARPS * 32) own_bf16<DP, 1, AttnTc<DP>::OWN_WARPS, 128>(pool, a, b - a.pre_blocks, smem);
-        return;
-    }
-    const AttnTask k = task_of<128>(pool, a, b);
-    if (k.begin >= k.end) { leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 320); return; }
-    attend_tc<DP>(pool, a, k, &tk, &tv, smem);
+    const AttnTask k = task_of<128>(pool, a, static_cast<int>(blockIdx.x));
+    if (k.begin < k.end) attend_tc<DP>(pool, a, k, &tk, &tv, smem);
+    else leave_nothing<bf16>(a, k, pool.dk, threadIdx.x, 320);
+    // the join waits for this kernel; with this it has waited for the one in front too
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 int paged_attn_device_error(int* code)
@@ -1250,7 +1246,7 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------- how the work is cut
-struct AttnPlan { bool tc, direct; int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps, block_warps; };
+struct AttnPlan { bool tc, direct; int rt, row_tiles, own_rows, own_tiles, pre_splits, own_splits, own_warps; };
 static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int heads, int prefix_stride, int table_stride)
 {
     AttnPlan p;
@@ -1264,7 +1260,6 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     p.own_rows = kv.dtype == 0 ? (m <= 4 ? 4 : p.rt) : p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
     p.row_tiles = static_cast<int>(std::max(1LL, ceil_div(rows, p.rt)));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
-    p.block_warps = !p.tc ? 4 : (kv.head_dim <= 64 ? AttnTc<64>::OWN_WARPS : AttnTc<128>::OWN_WARPS);
     const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
     const long long pre_units = static_cast<long long>(groups) * kv.kv_heads * p.row_tiles, own_units = static_cast<long long>(groups) * size * kv.kv_heads * p.own_tiles;
     // cached rows for a block when the tables are full: enough blocks for the machine a few times over, at least two steps each
@@ -1274,7 +1269,6 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
     if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / std::max(pre_units, 1LL), 1), ceil_div(pre, 512)));
     p.own_splits = static_cast<int>(ceil_div(own, chunk));
-    if (getenv("OC")) { long long oc = std::max(64LL, std::min(chunk, ceil_div(ceil_div(own_units * own, 148LL * 16 * atoi(getenv("OC"))), 64) * 64)); p.own_splits = static_cast<int>(ceil_div(own, oc)); }
     // a prefix and own rows of 128 at most: a block for both, without the join, takes 5.4 us where prefix, own rows and join take 7.6
     // (four beams of six heads behind 41 rows; behind 200 it would be 10.5 and 7.9)
     p.direct = !p.tc && pre > 0 && own > 0 && pre + own <= 128 && static_cast<long long>(groups) * size * kv.kv_heads <= 4 * 148;
@@ -1284,8 +1278,27 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
         p.pre_splits = 0;
         p.own_splits = 1;
     }
-    p.own_warps = kv.dtype == 0 || p.direct || ceil_div(own, std::max(1, p.own_splits)) > 512 ? p.block_warps : 1;
+    p.own_warps = kv.dtype == 0 || p.direct || ceil_div(own, std::max(1, p.own_splits)) > 512 ? 4 : 1;
     return p;
+}
+
+// a launch that may begin while the kernel in front of it runs (`early`)
+template <typename... P, typename... A>
+static int launch_behind(void (*kernel)(P...), unsigned blocks, int threads, int bytes, bool early, cudaStream_t s, const A&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = early ? 1 : 0;
+    NNB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+    NNB_LAUNCH_CHECK();
+    return 0;
 }
 
 template <typename T>
@@ -1302,16 +1315,18 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
     NNB_ARG_CHECK(pre_tasks + own_tasks <= INT_MAX, "too many queries for one call");
     a.pre_blocks = static_cast<int>(pre_tasks);
     a.tasks = static_cast<int>(pre_tasks + own_tasks);
-    const long long blocks = pre_tasks + ceil_div(own_tasks, p.block_warps / p.own_warps);
+    const long long blocks = pre_tasks + ceil_div(own_tasks, 4 / p.own_warps);
     a.c = 1.4426950408889634f / sqrtf(static_cast<float>(kv.head_dim));
     a.pairs = ((reinterpret_cast<uintptr_t>(a.q) & 3) == 0 && a.ldq % 2 == 0) ? 1 : 0;
     a.vectors = ((reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.ldq % 8 == 0) ? 1 : 0;
     a.stat = static_cast<float2*>(scratch);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + (rows * a.slots * 8 + 15) / 16 * 16);
     if (blocks > 0) {
+        a.first_block = p.tc ? a.pre_blocks : 0;
         auto go = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
             NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
-            kernel<<<static_cast<unsigned>(blocks), sizeof(T) == 4 ? kF32Threads : 128, bytes, s>>>(pool, a);
+            if (blocks == a.first_block) return 0;
+            kernel<<<static_cast<unsigned>(blocks - a.first_block), sizeof(T) == 4 ? kF32Threads : 128, bytes, s>>>(pool, a);
             NNB_LAUNCH_CHECK();
             return 0;
         };
@@ -1332,6 +1347,10 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
                 return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::smem(4), once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::smem(4), once[1]);
             }
         };
+        if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
+        else if (kv.head_dim <= 64) NNB_TRY(width(std::integral_constant<int, 64>()));
+        else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
+        else NNB_TRY(width(std::integral_constant<int, 256>()));
         if constexpr (sizeof(T) == 2) if (p.tc) {
             const long long pool_rows = static_cast<long long>(kv.pages) * kv.kv_heads * kv.page_size;
             CUtensorMap tk, tv;
@@ -1339,32 +1358,15 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
             NNB_TRY(tensor_map_2d(pool.v, kv.head_dim, pool_rows, kv.head_dim, 64, std::min(kv.page_size, 64), &tv, 2));
             auto tc = [&](auto* kernel, int bytes, PerDeviceOnce& once) {
                 NNB_TRY(once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }));
-                kernel<<<static_cast<unsigned>(blocks), 320, bytes, s>>>(pool, a, tk, tv);
-                NNB_LAUNCH_CHECK();
-                return 0;
+                return launch_behind(kernel, static_cast<unsigned>(a.pre_blocks), 320, bytes, own_tasks > 0, s, pool, a, tk, tv);
             };
             static PerDeviceOnce once[2];
-            if (kv.head_dim <= 64) NNB_TRY(tc(paged_attn_tc_kernel<64>, AttnTc<64>::SMEM, once[0]));
-            else NNB_TRY(tc(paged_attn_tc_kernel<128>, AttnTc<128>::SMEM, once[1]));
+            if (kv.head_dim <= 64) NNB_TRY(tc(paged_attn_tc_kernel<64>, AttnTc<64>::TILES, once[0]));
+            else NNB_TRY(tc(paged_attn_tc_kernel<128>, AttnTc<128>::TILES, once[1]));
         }
-        if (p.tc) {}
-        else if (kv.head_dim <= 32) NNB_TRY(width(std::integral_constant<int, 32>()));
-        else if (kv.head_dim <= 64) NNB_TRY(width(std::integral_constant<int, 64>()));
-        else if (kv.head_dim <= 128) NNB_TRY(width(std::integral_constant<int, 128>()));
-        else NNB_TRY(width(std::integral_constant<int, 256>()));
     }
     if (a.slots == 1) return 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows));
-    cfg.blockDim = dim3(128);
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = blocks > 0 ? 1 : 0;
-    NNB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T>, a, kv.head_dim));
-    NNB_LAUNCH_CHECK();
+    NNB_TRY(launch_behind(paged_attn_join_kernel<T>, static_cast<unsigned>(rows), 128, 0, blocks > 0, s, a, kv.head_dim));
     return 0;
 }
 

@@ -212,7 +212,7 @@ def test_attention_heads(g, dtype, heads, hk, dk, page, alibi):
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
-@pytest.mark.parametrize("size", [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 97, 130])
+@pytest.mark.parametrize("size", [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 97, 130, 161, 257])
 def test_attention_group_sizes(g, dtype, size):
     """One sequence to more than two tiles of them behind one prefix."""
     own = [(7 * i) % 23 - 1 for i in range(size)]
