@@ -1252,11 +1252,12 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     AttnPlan p;
     const int m = heads / kv.kv_heads;
     const long long rows = static_cast<long long>(size) * m;
-    // fp32 tiles take 16 query rows; bf16 streams 8 or 16; beyond that tcgen05 tiles take 128, and where a head is too wide
-    // for those mma.sync tiles take 64
-    p.tc = kv.dtype == 1 && rows > 64 && kv.head_dim <= 128 && prefix_stride > 0;
+    // bf16: warps stream up to 16 query rows; beyond that mma.sync tiles take 32 or 64 of heads up to 64 wide and the tcgen05
+    // tiles 128 of wider ones, or more of them (us, tcgen05 | mma.sync, heads of 64 behind 8192 rows and own ones: 20 rows 31 | 27.5,
+    // 64 rows 36 | 35; heads of 128 behind 32768: 32 rows 49 | 72, 64 rows 52 | 87); heads over 128 have only mma.sync tiles
+    p.tc = kv.dtype == 1 && rows > (kv.head_dim <= 64 ? 64 : 16) && kv.head_dim <= 128 && prefix_stride > 0;
     const int few = std::max<long long>(prefix_stride > 0 ? rows : 0, m) <= 4 ? 4 : (std::max<long long>(prefix_stride > 0 ? rows : 0, m) <= 8 ? 8 : 16);
-    p.rt = kv.dtype == 0 ? few : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 128 ? 32 : 64))));
+    p.rt = kv.dtype == 0 ? few : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 64 ? 32 : 64))));
     p.own_rows = kv.dtype == 0 ? (m <= 4 ? 4 : p.rt) : p.tc || (kv.dtype == 1 && (rows <= 8 || (m <= 8 && rows > 16))) ? 8 : 16;
     p.row_tiles = static_cast<int>(std::max(1LL, ceil_div(rows, p.rt)));
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
@@ -1342,8 +1343,8 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
             else {
                 const bool wide = p.own_rows == 16;
                 constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));
-                if (p.rt == 64) return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[3]);
-                if constexpr (DP < 256) if (p.rt == 32) return wide ? go(paged_attn_bf16_kernel<DP, 2, 2>, both, once[4]) : go(paged_attn_bf16_kernel<DP, 2, 1>, both, once[5]);
+                if constexpr (DP != 128) if (p.rt == 64) return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[3]);
+                if constexpr (DP <= 64) if (p.rt == 32) return wide ? go(paged_attn_bf16_kernel<DP, 2, 2>, both, once[4]) : go(paged_attn_bf16_kernel<DP, 2, 1>, both, once[5]);
                 return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::smem(4), once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::smem(4), once[1]);
             }
         };
