@@ -16,7 +16,8 @@ constexpr int kBatchPage = 16;                                  // rows of a pag
 struct BatchWs {
     size_t k, v, fixed, state, fresh, x, xn, qkv, att, mid, h1, h2, stat, scratch, scratch_bytes, total;
     int prompt_pages, own_pages;                                // pages of the prompt, of a sequence
-    // int32 arrays: prefix table | prefix length | position | row, each sequence's (fixed); table | spare page | length (state, fresh)
+    // int32 arrays: prefix table | prefix length | position | row, each sequence's | 0 .. seq - 1 | seq zeros (fixed);
+    // table | spare page | length (state, fresh)
     size_t fixed_ints, state_ints;
 };
 static nnb200_paged_kv batch_pool(const nnb200_gpt_config& c, const BatchWs& W, int seqs, uint8_t* ws)
@@ -39,7 +40,7 @@ static BatchWs batch_ws(const nnb200_gpt_config& c, int seqs, int new_rows)
     auto take = [&](size_t bytes) { const size_t o = off; off = (off + bytes + 255) / 256 * 256; return o; };
     const size_t pool = static_cast<size_t>(c.layers) * (W.prompt_pages + n * (W.own_pages + 1)) * kBatchPage * d * 4;
     W.k = take(pool); W.v = take(pool);
-    W.fixed_ints = W.prompt_pages + 1 + 2 * n + c.seq;
+    W.fixed_ints = W.prompt_pages + 1 + 2 * n + 2 * static_cast<size_t>(c.seq);
     W.state_ints = n * (W.own_pages + 2);
     W.fixed = take(W.fixed_ints * 4); W.state = take(W.state_ints * 4); W.fresh = take(W.state_ints * 4);
     W.x = take(n * d * 4); W.xn = take(n * d * 4); W.qkv = take(n * 3 * d * 4); W.att = take(n * d * 4); W.mid = take(n * d * 4);
@@ -52,14 +53,14 @@ static BatchWs batch_ws(const nnb200_gpt_config& c, int seqs, int new_rows)
     return W;
 }
 
-// page tables, spare pages and lengths of sequences without rows; sequence numbers of the prompt's rows are zero
+// page tables, spare pages and lengths of sequences without rows; row and sequence numbers to append the prompt by
 __global__ void batch_begin_kernel(int* fixed, int* state, int seqs, int prompt_pages, int own_pages, int prompt_len, int seq)
 {
     const int i0 = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
     for (int i = i0; i < prompt_pages; i += stride) fixed[i] = i;
     if (i0 == 0) fixed[prompt_pages] = prompt_len;
-    int* rows = fixed + prompt_pages + 1 + 2 * seqs;            // row numbers, to append the prompt by
-    for (int i = i0; i < seq; i += stride) rows[i] = i;
+    int* rows = fixed + prompt_pages + 1 + 2 * seqs;
+    for (int i = i0; i < seq; i += stride) { rows[i] = i; rows[seq + i] = 0; }
     for (int i = i0; i < seqs * own_pages; i += stride) state[i] = prompt_pages + i;
     for (int i = i0; i < seqs; i += stride) { state[seqs * own_pages + i] = prompt_pages + seqs * own_pages + i; state[seqs * (own_pages + 1) + i] = 0; }
 }
@@ -146,20 +147,14 @@ int nnb200_gpt_batch_begin(const nnb200_gpt_config* cfg, const void* decode_work
     int *fixed = reinterpret_cast<int*>(ws + W.fixed), *state = reinterpret_cast<int*>(ws + W.state), *rows = fixed + W.prompt_pages + 1 + 2 * seqs;
     batch_begin_kernel<<<static_cast<unsigned>(grid_for(std::max<long long>(W.fixed_ints, W.state_ints), 256)), 256, 0, s>>>(fixed, state, seqs, W.prompt_pages, W.own_pages, prompt_len, cfg->seq);
     NNB_LAUNCH_CHECK();
-    // The prompt's rows as the decode cache has them, already rotated: the prompt is a sequence of its own, whose page table's
-    // row is the prefix table.  Every row belongs to it; row numbers divided by seq are its number, 0.
+    // the prompt's rows as the decode cache has them, already rotated: the prompt is a sequence of its own, with the prefix table
+    // for a page table
     const int d = cfg->d_model;
     const float* cache = reinterpret_cast<const float*>(static_cast<const uint8_t*>(decode_workspace) + decode_cache(*cfg).kv);
-    NNB_CUDA_CHECK(cudaMemsetAsync(ws + W.fresh, 0, W.state_ints * 4, s));
     for (int l = 0; l < cfg->layers; ++l) {
         const float* k = cache + static_cast<size_t>(l) * 2 * cfg->seq * d;
-        for (int at = 0; at < prompt_len;) {
-            // sequence numbers are zeros, as many as there are at hand
-            const int n = static_cast<int>(std::min<long long>(prompt_len - at, static_cast<long long>(W.state_ints)));
-            NNB_TRY(nnb200_paged_append(&kv, l, nullptr, 0, nullptr, 0, k + static_cast<size_t>(at) * d, k + static_cast<size_t>(cfg->seq + at) * d, d, 0, n, 0,
-                                        reinterpret_cast<int*>(ws + W.fresh), rows + at, fixed, 1, W.prompt_pages, nullptr, 0, nullptr, s));
-            at += n;
-        }
+        NNB_TRY(nnb200_paged_append(&kv, l, nullptr, 0, nullptr, 0, k, k + static_cast<size_t>(cfg->seq) * d, d, 0, prompt_len, 0, rows + cfg->seq, rows, fixed, 1, W.prompt_pages,
+                                    nullptr, 0, nullptr, s));
     }
     return 0;
 }

@@ -220,6 +220,79 @@ def test_attention_group_sizes(g, dtype, size):
     _check_attention(g, dtype, 4, 1, 128, 32, 1, size, [130], own, seed=size, alibi=1)
 
 
+@pytest.mark.parametrize("heads,hk,dk,page,size", [(4, 4, 64, 8, 90), (2, 2, 40, 128, 70), (8, 2, 128, 256, 20), (6, 2, 96, 8, 40), (4, 1, 72, 64, 5), (3, 1, 256, 16, 30),
+                                                   (2, 2, 64, 256, 40), (32, 1, 128, 16, 9)])
+@pytest.mark.parametrize("alibi", [0, 1])
+def test_attention_many_rows(g, heads, hk, dk, page, size, alibi):
+    """Tiles of every kind with page sizes below, at and above their boxes, heads that pad them, odd strides and missing pages."""
+    prefix, own = [333, 128], [(11 * i) % 37 - 1 for i in range(2 * size)]
+    _check_attention(g, 1, heads, hk, dk, page, 2, size, prefix, own, alibi, seed=size)
+    _check_attention(g, 1, heads, hk, dk, page, 2, size, prefix, own, alibi, seed=size, ld_extra=3)
+
+    def change(q, kp, vp, ptab, otab, plen, olen):
+        ptab[0, min(1, ptab.shape[1] - 1)], ptab[1, 0], otab[3, 0] = -1, kp.shape[0], 2 ** 31 - 1
+        return q, kp, vp, ptab, otab, plen, olen
+    _check_attention(g, 1, heads, hk, dk, page, 2, size, prefix, own, alibi, seed=size, change=change)
+
+
+def test_attention_of_many_rows_large_scores_and_status_word(g):
+    _check_attention(g, 1, 4, 4, 64, 16, 1, 100, [1500], [(7 * i) % 50 for i in range(100)], seed=9, spread=60.0)
+    _check_attention(g, 1, 8, 2, 128, 32, 1, 30, [1500], [(7 * i) % 50 for i in range(30)], seed=9, spread=60.0)
+    assert g.gemm_status() == 0
+
+
+@pytest.mark.parametrize("heads,hk,dk,size", [(2, 2, 64, 80), (4, 1, 128, 40), (2, 2, 64, 30), (1, 1, 256, 20)])
+def test_attention_of_many_rows_meets_infinities(g, heads, hk, dk, size):
+    """A key of -inf has no weight, a value of +inf is one column's, a NaN key everybody's that sees it."""
+    import torch
+    q, kp, vp, ptab, otab, plen, olen = _attention_inputs(1, heads, hk, dk, 16, 2, size, [200, 77], [3] * (2 * size), 4)
+    q = np.abs(q) + 0.01
+    run = lambda k, v: _attention(g, 1, q, torch.from_numpy(k).cuda().bfloat16(), torch.from_numpy(v).cuda().bfloat16(), ptab, plen, otab, olen, size, 0)  # noqa: E731
+    clean, clean_lse, _ = run(kp, vp)
+    k2, v2 = kp.copy(), vp.copy()
+    k2[ptab[0, 2], :, 5] = -np.inf
+    v2[ptab[0, 0], :, 1, 7] = np.inf
+    got, lse, _ = run(k2, v2)
+    assert np.array_equal(got[size:], clean[size:]) and np.array_equal(lse[size:], clean_lse[size:])
+    assert np.all(got[:size, :, 7] == np.inf) and np.isfinite(np.delete(got[:size], 7, 2)).all() and np.all(lse[:size] < clean_lse[:size])
+    k2[ptab[0, 1], :, 0, 0] = np.nan
+    got, lse, _ = run(k2, vp)
+    assert np.isnan(got[:size]).all() and np.isnan(lse[:size]).all() and np.array_equal(got[size:], clean[size:])
+    got, lse, _ = run(np.where(np.isnan(kp), kp, -np.inf).astype(np.float32), vp)
+    assert np.all(got == 0) and np.all(np.isneginf(lse))
+
+
+def test_attention_on_two_streams_at_once(g):
+    """Two calls that may overlap, each with a scratch of its own; tensors made on one stream and used on another behind it."""
+    import torch
+    cases = []
+    for seed, (heads, hk, dk, size) in enumerate([(4, 4, 64, 90), (8, 2, 128, 3)]):
+        q, kp, vp, ptab, otab, plen, olen = _attention_inputs(1, heads, hk, dk, 16, 2, size, [700, 333], [(13 * i) % 60 - 1 for i in range(2 * size)], seed)
+        n = 2 * size
+        t = dict(q=torch.from_numpy(q.reshape(n, -1)).cuda().bfloat16(), k=torch.from_numpy(kp).cuda().bfloat16(), v=torch.from_numpy(vp).cuda().bfloat16(), size=size, heads=heads)
+        t.update(pt=g.dev(ptab), pl=g.dev(plen), ot=g.dev(otab), ol=g.dev(olen), out=torch.zeros((n, heads * dk), device="cuda", dtype=torch.bfloat16))
+        t["kv"] = _descr(g, t["k"], t["v"], 16, 1)
+        t["need"] = g.call("nnb200_paged_attention_scratch_bytes", C.byref(t["kv"]), 2, size, heads, ptab.shape[1], otab.shape[1])
+        t["scratch"] = torch.empty(t["need"], dtype=torch.uint8, device="cuda")
+        cases.append(t)
+
+    def run(t):
+        ld = t["q"].shape[1]
+        g.call("nnb200_paged_attention", C.byref(t["kv"]), 0, g.ptr(t["q"]), ld, g.ptr(t["out"]), ld, None, g.ptr(t["pt"]), t["pt"].shape[1], g.ptr(t["pl"]), g.ptr(t["ot"]),
+               t["ot"].shape[1], g.ptr(t["ol"]), 2, t["size"], t["heads"], 0, g.ptr(t["scratch"]), t["need"], g.stream())
+        return t["out"]
+    want = [run(t).clone() for t in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(20):
+        for s, t in zip(streams, cases):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                run(t)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t["out"], w) for t, w in zip(cases, want))
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("prefix", [1, 7, 8, 63, 64, 65, 127, 128, 129, 1000, 4097])
 def test_attention_prefix_lengths(g, dtype, prefix):
