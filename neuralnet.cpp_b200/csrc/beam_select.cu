@@ -7,11 +7,12 @@
 // continuations of two beams come closer than that, which happens to one group in some hundreds, their beams' normalisers
 // are computed again in 64 bits, as sums of whole numbers: exact to 1e-12, and the same in whatever order a row holds its logits.
 //
-// Two kernels.  The first reads the logits once, bound by memory: a block per span of a row sums its exponentials and keeps its n
-// best (value, token) pairs.  The order within a row does not depend on the normaliser, so that needs no second pass.  What
-// makes it one pass is a threshold: n values are known to be at least as large, so that only larger ones, few after the first
-// tile of a row, go to a list in shared memory.  The second, already resident when the first ends, joins the spans' sums
-// and picks from the rows' lists.
+// Two kernels.  The first reads the logits once, bound by memory and the exponentials: a block per span of a row sums its
+// exponentials and keeps the maximum of each thread's share of each tile.  The order within a row does not depend on the
+// normaliser, so its n best can be had from these: n threads' maxima bound them from below, and only the few shares that reach the
+// bound are looked at again.  (Comparing each logit with a running threshold on the way took 2000 of a tile's 3800 clocks: with
+// 1000 logits a warp and tile somebody always has one.)  The second kernel, already resident when the first ends, joins the spans'
+// sums and picks from the rows' lists.
 #include <algorithm>
 
 #include "common.cuh"
@@ -25,6 +26,8 @@ constexpr int kSelPer = 32, kSelTile = kSelThreads * kSelPer;   // logits of a t
 constexpr int kSelMost = 128;                                   // continuations of a group
 constexpr int kSelSlack = 256;                                  // a list this much longer than n is cut back to n
 constexpr int kSelList = kSelTile + kSelMost + kSelSlack;       // a tile may go into the list whole
+constexpr int kSelTiles = 16;                                   // tiles of a span at most
+constexpr int kSelPieces = kSelList / kSelPer - 4;              // threads' shares of tiles that may go into the list together
 
 struct alignas(16) SpanSum { double sum; float ref; };          // of exponentials against the reference point
 
@@ -104,8 +107,8 @@ struct SelectShared {
     Entry best[kSelMost];
     uint32_t sw[kSelWarps][2];
     double sum[kSelWarps];
-    float ref[kSelWarps];
-    int count;
+    float ref[kSelWarps], top[kSelTiles][kSelThreads];          // top: maximum of each thread's share of each tile
+    int count, pieces, piece[kSelPieces > kSelThreads ? kSelPieces : kSelThreads];
 };
 
 // Cuts the list back to its n best, sorted; sh.count entries before, returns how many after (all threads call it).
@@ -174,14 +177,12 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
     if (a.ended && a.ended[row]) return;                        // its only continuation is not in its logits
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     const int begin = part * a.span, end = min(begin + a.span, a.vocab);
-    if (threadIdx.x == 0) sh.count = 0;
-    __syncthreads();
+    if (threadIdx.x == 0) { sh.count = 0; sh.pieces = 0; }
     constexpr int N = Vec16<T>::N, VECS = kSelPer / N;
     // exponentials are taken against the first tile's maximum, or one of this thread's own where that is far behind
-    float ref = -INFINITY;
+    float ref = -INFINITY, most = -INFINITY;
     double sum = 0.0;
-    float most = -INFINITY, least = 0.f;                        // the thread's maximum; what can still be among the n best
-    int left = -1;                                              // entries of the list when it was cut last: all of them, sorted, if no more came
+    const int tiles = (end - begin + kSelTile - 1) / kSelTile;
     // whole tiles of aligned rows are read a tile ahead
     Vec16<T> raw[VECS];
     auto whole = [&](int t0) { return a.vectors && t0 + kSelTile <= end; };
@@ -190,27 +191,30 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
 #pragma unroll
         for (int i = 0; i < VECS; ++i) raw[i] = ld16(x + t0 + (i * kSelThreads + static_cast<int>(threadIdx.x)) * N);
     };
+    // logit j of thread t in the tile at t0: vectors of neighbours lie side by side
+    auto token_of = [&](int t0, int t, int j) { return a.vectors ? t0 + (j / N * kSelThreads + t) * N + j % N : t0 + j * kSelThreads + t; };
     ahead(begin);
-    for (int t0 = begin; t0 < end; t0 += kSelTile) {
+    for (int i = 0; i < tiles; ++i) {
+        const int t0 = begin + i * kSelTile;
         float v[kSelPer];
-        // logit j of this thread is token_of(j): vectors of neighbours lie side by side
-        auto token_of = [&](int j) { return a.vectors ? t0 + (j / N * kSelThreads + static_cast<int>(threadIdx.x)) * N + j % N : t0 + j * kSelThreads + static_cast<int>(threadIdx.x); };
         if (whole(t0)) {
 #pragma unroll
             for (int j = 0; j < kSelPer; ++j) v[j] = to_f32(raw[j / N].v[j % N]);
             ahead(t0 + kSelTile);
         } else {
 #pragma unroll
-            for (int j = 0; j < kSelPer; ++j) { const int t = token_of(j); v[j] = t < end ? to_f32(x[t]) : -INFINITY; }
+            for (int j = 0; j < kSelPer; ++j) { const int t = token_of(t0, threadIdx.x, j); v[j] = t < end ? to_f32(x[t]) : -INFINITY; }
         }
-        float top = v[0];
+        float top4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int j = 1; j < kSelPer; ++j) top = fmaxf(top, v[j]);
-        const bool first = t0 == begin;
-        if (first) {
+        for (int j = 4; j < kSelPer; ++j) top4[j & 3] = fmaxf(top4[j & 3], v[j]);
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        sh.top[i][threadIdx.x] = top;
+        most = fmaxf(most, top);
+        if (i == 0) {
             ref = warp_max(top);
             if (lane == 0) sh.ref[warp] = ref;
-            least = value_of(max(bound_for<kSelWarps>(order_of(top), a.n, sh.sw), order_of(-INFINITY) + 1));
+            __syncthreads();
 #pragma unroll
             for (int w = 0; w < kSelWarps; ++w) ref = fmaxf(ref, sh.ref[w]);
         }
@@ -221,36 +225,46 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
 #pragma unroll
         for (int h = 0; h < 4; ++h) part[h] = exps_against(v + 8 * h, minus_ref);
         sum += static_cast<double>((part[0] + part[1]) + (part[2] + part[3]));
-        if (top >= least) {
-            // few of a warp's logits get here, and not often: they are read again, by number
-            uint32_t hits = 0;
-#pragma unroll
-            for (int j = 0; j < kSelPer; ++j) hits |= v[j] >= least ? 1u << j : 0u;
-            int at = atomicAdd(&sh.count, __popc(hits));
-            for (; hits; hits &= hits - 1) { const int t = token_of(__ffs(hits) - 1); sh.list[at++] = entry_of(to_f32(x[t]), t); }
-        }
-        // thread maxima so far bound what is to come; worth its time when twice as much has been seen
-        most = fmaxf(most, top);
-        const int seen = (t0 - begin) / kSelTile + 1;
-        uint32_t bound = 0;
-        if (!first && (seen & (seen - 1)) == 0 && t0 + kSelTile < end) bound = bound_for<kSelWarps>(order_of(most), a.n, sh.sw);
-        __syncthreads();
-        const int count = sh.count;
-        if (first || count > a.n + kSelSlack) {
-            // from the n-th best up, but not equal to it: an equal one comes later in the row
-            left = cut_list(sh, a.n);
-            least = value_of((left == a.n ? static_cast<uint32_t>(sh.list[a.n - 1] >> 32) : order_of(-INFINITY)) + 1);
-        }
-        if (bound) least = fmaxf(least, value_of(bound + 1));
-        if (t0 + kSelTile < end) __syncthreads();
     }
+    // the shares that hold one of the n best, one warp each
+    float least = value_of(max(bound_for<kSelWarps>(order_of(most), a.n, sh.sw), order_of(-INFINITY) + 1));
+    auto look = [&](int pieces) {
+        for (int p = warp; p < pieces; p += kSelWarps) {
+            const int t = token_of(begin + (sh.piece[p] >> 8) * kSelTile, sh.piece[p] & 255, lane);
+            const float v = t < end ? to_f32(x[t]) : -INFINITY;
+            if (v >= least) sh.list[atomicAdd(&sh.count, 1)] = entry_of(v, t);
+        }
+    };
+    static_assert(kSelPer == 32 && kSelThreads <= 256, "a lane for each logit of a share");
+    int mine = 0;
+    for (int i = 0; i < tiles; ++i) mine += sh.top[i][threadIdx.x] >= least;
+    if (mine) {
+        int at = atomicAdd(&sh.pieces, mine);
+        for (int i = 0; i < tiles; ++i)
+            if (sh.top[i][threadIdx.x] >= least) { if (at < kSelPieces) sh.piece[at] = i << 8 | static_cast<int>(threadIdx.x); ++at; }
+    }
+    __syncthreads();
+    if (sh.pieces <= kSelPieces) look(sh.pieces);
+    else {
+        // many equal values: tile by tile, in order, the list cut back on the way; what equals the n-th best comes too late from then on
+        for (int i = 0; i < tiles; ++i) {
+            __syncthreads();
+            if (threadIdx.x == 0) sh.pieces = 0;
+            __syncthreads();
+            if (sh.top[i][threadIdx.x] >= least) sh.piece[atomicAdd(&sh.pieces, 1)] = i << 8 | static_cast<int>(threadIdx.x);
+            __syncthreads();
+            look(sh.pieces);
+            __syncthreads();
+            if (sh.count > a.n + kSelSlack && cut_list(sh, a.n) == a.n) least = fmaxf(least, value_of(static_cast<uint32_t>(sh.list[a.n - 1] >> 32) + 1));
+        }
+    }
+    const int left = cut_list(sh, a.n);
     // the block's sum, against the largest of the threads' points
     float m = ref;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) sh.ref[warp] = m;
     __syncthreads();
-    if (sh.count != left) left = cut_list(sh, a.n);
     m = sh.ref[0];
 #pragma unroll
     for (int w = 1; w < kSelWarps; ++w) m = fmaxf(m, sh.ref[w]);
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(W * 32) select_pick_kernel(const __grid_consta
 static int select_spans(int groups, int beams, int vocab)
 {
     const long long rows = std::max(1LL, static_cast<long long>(groups) * beams), tiles = ceil_div(vocab, kSelTile);
-    const long long want = std::max<long long>(1, 148 * 4 / rows), per = ceil_div(tiles, std::min(tiles, want));
+    const long long want = std::max<long long>(1, 148 * 4 / rows), per = std::min<long long>(ceil_div(tiles, std::min(tiles, want)), kSelTiles);
     return static_cast<int>(ceil_div(tiles, per));
 }
 
