@@ -127,11 +127,12 @@ __device__ int cut_list(SelectShared& sh, int n)
         for (int i = threadIdx.x; i < count; i += kSelThreads) { const Entry e = sh.list[i]; if (e >> 32 == bound >> 32) tie = max(tie, static_cast<uint32_t>(e)); }
         __syncthreads();
         bound |= bound_for<kSelWarps>(tie, n, sh.sw);
-        uint32_t keep = 0;
+        unsigned long long keep = 0;
+        static_assert(PER <= 64, "a bit for each of a thread's entries");
 #pragma unroll 1
         for (int j = 0; j < PER; ++j) {
             const int i = threadIdx.x + j * kSelThreads;
-            if (i < count && sh.list[i] >= bound) keep |= 1u << j;
+            if (i < count && sh.list[i] >= bound) keep |= 1ull << j;
         }
         if (__syncthreads_count(keep != 0) == 0) break;
         if (threadIdx.x == 0) sh.count = 0;
@@ -140,7 +141,7 @@ __device__ int cut_list(SelectShared& sh, int n)
 #pragma unroll 1
         for (int j = 0; j * kSelThreads < count; ++j) {
             const int i = threadIdx.x + j * kSelThreads;
-            const bool k = keep >> j & 1u;
+            const bool k = keep >> j & 1ull;
             const Entry e = k ? sh.list[i] : 0;
             __syncthreads();
             if (k) sh.list[atomicAdd(&sh.count, 1)] = e;
@@ -229,19 +230,28 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
     // the shares that hold one of the n best, one warp each
     float least = value_of(max(bound_for<kSelWarps>(order_of(most), a.n, sh.sw), order_of(-INFINITY) + 1));
     auto look = [&](int pieces) {
-        for (int p = warp; p < pieces; p += kSelWarps) {
-            const int t = token_of(begin + (sh.piece[p] >> 8) * kSelTile, sh.piece[p] & 255, lane);
-            const float v = t < end ? to_f32(x[t]) : -INFINITY;
-            if (v >= least) sh.list[atomicAdd(&sh.count, 1)] = entry_of(v, t);
+        for (int p0 = warp; p0 < pieces; p0 += 4 * kSelWarps) {  // four of a warp's on their way at a time
+            int t[4];
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int piece = sh.piece[min(p0 + u * kSelWarps, pieces - 1)];
+                t[u] = token_of(begin + (piece >> 8) * kSelTile, piece & 255, lane);
+                v[u] = p0 + u * kSelWarps < pieces && t[u] < end ? to_f32(x[t[u]]) : -INFINITY;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (v[u] >= least) sh.list[atomicAdd(&sh.count, 1)] = entry_of(v[u], t[u]);
         }
     };
     static_assert(kSelPer == 32 && kSelThreads <= 256, "a lane for each logit of a share");
-    int mine = 0;
-    for (int i = 0; i < tiles; ++i) mine += sh.top[i][threadIdx.x] >= least;
-    if (mine) {
-        int at = atomicAdd(&sh.pieces, mine);
-        for (int i = 0; i < tiles; ++i)
-            if (sh.top[i][threadIdx.x] >= least) { if (at < kSelPieces) sh.piece[at] = i << 8 | static_cast<int>(threadIdx.x); ++at; }
+    uint32_t reach = 0;
+#pragma unroll
+    for (int i = 0; i < kSelTiles; ++i) reach |= i < tiles && sh.top[i][threadIdx.x] >= least ? 1u << i : 0;
+    static_assert(kSelTiles <= 32, "a bit for each tile");
+    if (reach) {
+        for (int at = atomicAdd(&sh.pieces, __popc(reach)); reach && at < kSelPieces; ++at, reach &= reach - 1)
+            sh.piece[at] = (__ffs(reach) - 1) << 8 | static_cast<int>(threadIdx.x);
     }
     __syncthreads();
     if (sh.pieces <= kSelPieces) look(sh.pieces);
@@ -385,11 +395,13 @@ __global__ void __launch_bounds__(W * 32) select_pick_kernel(const __grid_consta
     for (int b = warp; b < a.beams; b += W) {           // a warp per beam
         if (sh.ended[b]) { if (lane == 0) sh.norm[b] = NAN; continue; }
         const SpanSum* st = a.stat + static_cast<long long>(g * a.beams + b) * a.spans;
-        float m = -INFINITY;
-        for (int i = lane; i < a.spans; i += 32) m = fmaxf(m, st[i].ref);
+        const SpanSum own = lane < a.spans ? st[lane] : SpanSum{0.0, -INFINITY};
+        float m = own.ref;
+        for (int i = lane + 32; i < a.spans; i += 32) m = fmaxf(m, st[i].ref);
         m = warp_max(m);
-        double s = 0.0;
-        for (int i = lane; i < a.spans; i += 32) s += st[i].ref == -INFINITY ? st[i].sum : (st[i].ref == m ? st[i].sum : st[i].sum * exp(static_cast<double>(st[i].ref) - m));
+        auto against = [&](const SpanSum& x) { return x.ref == -INFINITY || x.ref == m ? x.sum : x.sum * exp(static_cast<double>(x.ref) - m); };
+        double s = against(own);
+        for (int i = lane + 32; i < a.spans; i += 32) s += against(st[i]);
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         // NaN from a NaN or +inf logit; a row of -inf has no maximum
         if (lane == 0) sh.norm[b] = m == -INFINITY ? static_cast<double>(NAN) : static_cast<double>(m) + log(s);

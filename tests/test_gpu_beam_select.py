@@ -144,3 +144,14 @@ def test_select_says_which_of_close_candidates_is_better(g):
         s = np.float32(norm[1] - norm[0])
         scores = np.array([[0.0, float(s) + 2.0 ** -20 * (1 if seed % 2 else -1)]])
         _check(g, 0, x.astype(np.float32)[None], scores, None, -1, 30)
+
+
+def test_select_more_candidates_than_a_tile_of_a_long_row(g):
+    """Rows whose first tile of 4096 is one value and whose second lies above it but for some tokens, of which the best are spread."""
+    groups, vocab, n = 600, 8192, 128
+    logits = np.ones((groups, 1, vocab), dtype=np.float32)
+    second = np.full((8, 128, 4), 2.0, dtype=np.float32)
+    second[0, :, 0] = 3.0
+    second[:, 127] = 1.0
+    logits[:, 0, 4096:] = second.reshape(-1)
+    _check(g, 0, logits, np.zeros((groups, 1)), None, -1, n)
