@@ -982,16 +982,25 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
             if (!pair_any(quad, bad)) {
                 l += sL[(half ^ 1) * 128 + row];
                 tc_fence_after();
+                // through shared memory (the last products have read K and V), so that a row is written by neighbouring threads
+                constexpr int VECS = DP / 8, ROWS = 32 / VECS;  // 16 bytes at a time: a warp's half of a row, rows at a time
+                static_assert(8 * 32 * VECS * 16 <= 2 * ST * Tc::TILE, "the sums fit the tiles");
+                uint8_t* stage = sK + (warp - 2) * 32 * VECS * 16;
 #pragma unroll 1
                 for (int c = 0; c < DP / 2; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(tmem_o + lanes + half * (DP / 2) + c, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        if (live && half * (DP / 2) + c + j < dk)
-                            leave<bf16>(a, k, dk, row, half * (DP / 2) + c + j,
-                                        make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3])), m, l);
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(stage + (lane * VECS + (((c + j) / 4) ^ sw)) * 16) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
+                __syncwarp();
+#pragma unroll 2
+                for (int r0 = 0; r0 < 32; r0 += ROWS) {
+                    const int r = r0 + lane / VECS, v = lane % VECS, c = half * (DP / 2) + v * 4;
+                    const float4 o = *reinterpret_cast<const float4*>(stage + (r * VECS + (v ^ (r & 7))) * 16);
+                    const float mr = __shfl_sync(0xffffffffu, m, r), lr = __shfl_sync(0xffffffffu, l, r);
+                    if (quad * 32 + r < k.rows && c < dk) leave<bf16>(a, k, dk, quad * 32 + r, c, o, mr, lr);
                 }
             }
         }
@@ -1210,23 +1219,38 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
     const int seq = a.by_heads.split(h), slots = a.slots;
     const bool live = sees(a, seq);
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int vecs = dk / 4, sets = a.by_vecs.div(128), set = a.by_vecs.div(threadIdx.x), c = (threadIdx.x - set * vecs) * 4;
     const float2* st = a.stat + row * slots;
+    const float* part = a.part + row * slots * dk + c;
+    // a thread's first places are under way before their maximum is known
+    constexpr int AHEAD = 4;
+    float2 s[AHEAD];
+    float4 y[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+        const int i = set + u * sets;
+        const bool there = set < sets && i < slots;
+        s[u] = there ? st[i] : make_float2(-INFINITY, 0.f);
+        y[u] = there ? *reinterpret_cast<const float4*>(part + static_cast<long long>(i) * dk) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     float m = -INFINITY;
-    for (int i = threadIdx.x; i < slots; i += 128) m = fmaxf(m, st[i].x);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) m = fmaxf(m, s[u].x);
+    for (int i = AHEAD * sets + threadIdx.x; i < slots; i += 128) m = fmaxf(m, st[i].x);
     m = block_max(m, red);
     const float ref = m == -INFINITY ? 0.f : m;
-    const int vecs = dk / 4, sets = a.by_vecs.div(128), set = a.by_vecs.div(threadIdx.x), c = (threadIdx.x - set * vecs) * 4;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
+    auto add = [&](const float2& s, const float4& y) {
+        if (s.y == 0.f) return;                                 // nothing was left there, not even sums
+        const float e = exp2f(s.x - ref);
+        l = fmaf(s.y, e, l);
+        x.x = fmaf(y.x, e, x.x); x.y = fmaf(y.y, e, x.y); x.z = fmaf(y.z, e, x.z); x.w = fmaf(y.w, e, x.w);
+    };
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) add(s[u], y[u]);
     if (set < sets)
-        for (int i = set; i < slots; i += sets) {
-            const float2 s = st[i];
-            if (s.y == 0.f) continue;                           // nothing was left there, not even sums
-            const float e = exp2f(s.x - ref);
-            const float4 y = *reinterpret_cast<const float4*>(a.part + (row * slots + i) * dk + c);
-            l = fmaf(s.y, e, l);
-            x.x = fmaf(y.x, e, x.x); x.y = fmaf(y.y, e, x.y); x.z = fmaf(y.z, e, x.z); x.w = fmaf(y.w, e, x.w);
-        }
+        for (int i = set + AHEAD * sets; i < slots; i += sets) add(st[i], *reinterpret_cast<const float4*>(part + static_cast<long long>(i) * dk));
     *reinterpret_cast<float4*>(sx + threadIdx.x * 4) = x;
     sl[threadIdx.x] = l;
     __syncthreads();
