@@ -669,12 +669,13 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
 //   warp 0     looks up the step's pages and loads their rows by TMA, a box of a page (64 rows of a larger one) per lane; pages
 //              that are not there are loaded from behind the pool's end, where TMA fills in zeros
 //   warp 1     issues the products: S, and O += P V in two halves of 64 cached rows
-//   warps 2-9  two threads per query row, half of the columns each: read their 64 scores, make P (bf16, shared memory, 64 cached
-//              rows at a time) with the reference point of the exponentials moved, and O rescaled, only when a score is more
-//              than 2^8 above it (the one thing the two must agree on); V's rows behind the end are zeroed by these warps
+//   warps 2-9  two threads per query row, half of the columns each: read their 64 scores, make P (bf16, over the scores, for 64
+//              cached rows at a time) with the reference point of the exponentials moved, and O rescaled, only when a score is
+//              more than 2^8 above it (the one thing the two must agree on); V's rows behind the end are zeroed by these warps
 //              before P is handed over, because a page's unused rows may hold anything
-// A step is a chain - S, maximum, exponentials, P, P V - with the next step's S between the two halves; two blocks an SM overlap
-// two chains.  64 cached rows a step instead (an S of 128 x 64 takes the tensor core as long as one of 128 x 128) had the issue
+// A step is a chain - S, maximum, exponentials, P, P V; two blocks an SM overlap two chains.  P stands in TMEM where its scores
+// stood: with P in shared memory the products' operands, P and the arriving tiles asked for 3600 clocks of shared memory's
+// bandwidth a step of both blocks, of 4200 that it took, although the next step's S could then start half a P V earlier.  64 cached rows a step instead (an S of 128 x 64 takes the tensor core as long as one of 128 x 128) had the issue
 // of products as its bound: 2400 clocks for 64 rows and block, 12 products of 130 clocks.
 // Every wait is bounded; one that gives up raises a status word, the others see it, and the block drains: the two threads of a
 // row leave together, at the barrier where they compare notes.
@@ -684,7 +685,7 @@ template <int DP> struct AttnTc {
     static constexpr int NS = DP / 64, ST = DP == 64 ? 2 : 1, KT = 128;
     static constexpr int SUB = 128 * 128;                       // bytes of 128 rows by 64 columns
     static constexpr int TILE = NS * SUB;
-    static constexpr int OFF_K = TILE, OFF_V = OFF_K + ST * TILE, OFF_P = OFF_V + ST * TILE, OFF_X = OFF_P + SUB, OFF_BAR = OFF_X + 2 * 128 * 2;
+    static constexpr int OFF_K = TILE, OFF_V = OFF_K + ST * TILE, OFF_X = OFF_V + ST * TILE, OFF_BAR = OFF_X + 2 * 128 * 2;
     static constexpr int TILES = OFF_BAR + 256;                 // DP = 128: two blocks fit an SM, with 256 bytes to spare
     static constexpr uint32_t TMEM_COLS = 256;                  // scores [0, 128), O [128, 128 + DP)
 };
@@ -708,13 +709,13 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
 {
     using Tc = AttnTc<DP>;
     constexpr int ST = Tc::ST, NS = Tc::NS, KT = Tc::KT;
-    uint8_t *sQ = smem, *sK = smem + Tc::OFF_K, *sV = smem + Tc::OFF_V, *sP = smem + Tc::OFF_P;
+    uint8_t *sQ = smem, *sK = smem + Tc::OFF_K, *sV = smem + Tc::OFF_V;
     bf16* sX = reinterpret_cast<bf16*>(smem + Tc::OFF_X);       // (half, row)
     float* sL = reinterpret_cast<float*>(sQ);                   // (half, row), once the query tile has been used
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tc::OFF_BAR);
     const uint32_t bar0 = smem_u32(bars);
-    const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST, s_free = s_full + 8,
-                   p_full = s_full + 16, pv_done = s_full + 24, q_full = s_full + 32;
+    const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST,
+                   p_full = s_full + 8, pv_done = s_full + 24, q_full = s_full + 32;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * ST + 5);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dk = pool.dk, ps = 1 << pool.page_shift;
@@ -723,7 +724,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 1); mbar_init(v_empty + 8 * i, 1); }
-        mbar_init(s_full, 1); mbar_init(s_free, 8); mbar_init(p_full, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8);
+        mbar_init(s_full, 1); mbar_init(p_full, 8); mbar_init(p_full + 8, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8);
         *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;         // the swizzled tiles need a 1024-byte aligned base
         if (*abort_flag) atomicCAS(&g_paged_attn_error, 0, 9 << 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -780,7 +781,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     } else if (warp == 1) {
         if (lane == 0) {
             bool ok = !*abort_flag && wait(q_full, 0, 5);
-            const uint64_t dq = smem_desc(smem_u32(sQ), 16, 1024), dkey = smem_desc(smem_u32(sK), 16, 1024), dp = smem_desc(smem_u32(sP), 16, 1024),
+            const uint64_t dq = smem_desc(smem_u32(sQ), 16, 1024), dkey = smem_desc(smem_u32(sK), 16, 1024),
                            dv = smem_desc(smem_u32(sV), Tc::SUB, 1024);          // addresses in units of 16 bytes: offsets are added below
             auto issue_s = [&](int i) -> bool {
                 const int st = i % ST;
@@ -797,12 +798,11 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
             };
             auto issue_pv = [&](int i, int part) -> bool {
                 const int st = i % ST;
-                if (!wait(p_full, 2 * i + part, 7)) return false;
+                if (!wait(p_full + 8 * part, i, 7)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    umma_bf16(tmem_o, dp + (x * 32 >> 4), dv + (st * Tc::TILE >> 4) + ((part * 4 + x) * 2048 >> 4), IDESC_PV, i > 0 || part > 0 || x > 0 ? 1u : 0u);
-                umma_commit(pv_done);
+                    umma_bf16_ta(tmem_o, tmem + part * 64 + (x >> 1) * 32 + (x & 1) * 8, dv + (st * Tc::TILE >> 4) + ((part * 4 + x) * 2048 >> 4), IDESC_PV, i > 0 || part > 0 || x > 0 ? 1u : 0u);
                 return true;
             };
             if (ok) ok = issue_s(0);
@@ -810,19 +810,20 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                 const int st = i % ST;
                 if (!(ok = wait(v_full + 8 * st, i / ST, 8))) break;
                 if (!(ok = issue_pv(i, 0))) break;
-                if (i + 1 < steps) {
-                    if (!(ok = wait(s_free, i, 15))) break;     // the scores of step i are read
-                    if (!(ok = issue_s(i + 1))) break;
-                }
                 if (!(ok = issue_pv(i, 1))) break;
+                umma_commit(pv_done);
                 umma_commit(v_empty + 8 * st);
+                if (i + 1 == steps) break;
+                // the next scores take the columns of this step's, where P stands
+                if (!(ok = wait(pv_done, i, 15))) break;
+                if (!(ok = issue_s(i + 1))) break;
             }
         }
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const int sw = row & 7;
-        const bool live = row < k.rows, work = quad * 32 < k.rows;   // warps without rows hand over zeros
+        const bool live = row < k.rows, work = quad * 32 < k.rows;   // of a warp without rows the scores serve as P: its rows of O are nobody's
         const AttnRow w = row_of(a, k, live ? row : 0);
         {   // half of the query row, zero where there is none
             const bf16* q = static_cast<const bf16*>(a.q) + w.seq * a.ldq + static_cast<long long>(w.head) * dk;
@@ -841,11 +842,6 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                 }
                 *reinterpret_cast<uint4*>(sQ + (cc >> 3) * Tc::SUB + row * 128 + (((cc & 7) ^ sw) << 4)) = v;
             }
-        }
-        uint8_t* prow = sP + row * 128;
-        if (!work) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(prow + (half * 4 + c) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -920,9 +916,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                     const float back = move ? exp2_fast(m - top) : 1.0f;          // 0 from -inf
                     if (move) m = top;
                     l *= back;
-                    if (i > 0) {
-                        bad |= !wait_all(pv_done, 2 * i - 1, 12);
-                        tc_fence_after();
+                    if (i > 0) {                                // the products of the step before are in: this one's scores came after them
 #pragma unroll 1
                         for (int c = 0; c < DP / 2; c += 32) {
                             uint32_t r[32];
@@ -945,11 +939,6 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                 if (work) {
                     float x[32];
                     scores(p, x);
-                    if (p == 1) {                               // the scores are in registers: their columns go back to the tensor core
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(s_free);
-                    }
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         float e0, e1;
@@ -960,16 +949,13 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                         else sum0 = add2(sum0, pack2(e0, e1));
                         pk[j] = pack_bf16x2(e0, e1);            // rounded for the tensor cores, summed as they are
                     }
-                } else if (p == 1 && lane == 0) mbar_arrive(s_free);
-                if (i + p > 0) bad |= !wait_all(pv_done, 2 * i + p - 1, 13);      // the P before has been used
-                if (work) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(prow + (((half * 4 + c) ^ sw) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+                    tmem_st16(tmem + lanes + p * 64 + half * 32, pk);   // over scores that only this warp reads, and has read
+                    tmem_st_wait();
                 }
                 tc_fence_before();
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full);
+                if (lane == 0) mbar_arrive(p_full + 8 * p);        // a barrier for each part: a warp may be done with both before others with one
             }
             float s0, s1;
             unpack2(add2(sum0, sum1), s0, s1);
@@ -977,7 +963,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
             if (!work && bad) break;
         }
         if (work) {
-            bad |= !wait_all(pv_done, 2 * steps - 1, 14);
+            bad |= !wait_all(pv_done, steps - 1, 14);
             sL[half * 128 + row] = l;
             if (!pair_any(quad, bad)) {
                 l += sL[(half ^ 1) * 128 + row];
