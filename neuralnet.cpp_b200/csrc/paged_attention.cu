@@ -893,19 +893,47 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                     for (int j = 0; j < 32; ++j) if (!(there[p] >> j & 1u)) x[j] = -INFINITY;
                 }
             };
+            float x[32];
+            uint32_t pk[16];
+            uint64_t sum0 = 0ull, sum1 = 0ull;
+            auto most = [&](const float (&x)[32]) -> float {
+                float top4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int j = 4; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
+                return fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+            };
+            auto exponentials = [&](const float (&x)[32]) {
+                const float ref = m == -INFINITY ? 0.f : m;
+                const uint64_t mul_2 = pack2(mul, mul), ref_2 = pack2(-ref, -ref);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float e0, e1;
+                    unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul_2, ref_2), e0, e1);
+                    e0 = exp2_fast(e0);
+                    e1 = exp2_fast(e1);
+                    if (j & 1) sum1 = add2(sum1, pack2(e0, e1));
+                    else sum0 = add2(sum0, pack2(e0, e1));
+                    pk[j] = pack_bf16x2(e0, e1);                // rounded for the tensor cores, summed as they are
+                }
+            };
+            auto hand_over = [&](int p) {
+                if (work) {
+                    tmem_st16(tmem + lanes + p * 64 + half * 32, pk);   // over scores that only this warp reads, and has read
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * p);     // a barrier for each part: a warp may be done with both before others with one
+            };
             if (work) {
                 tc_fence_after();
-                float top = -INFINITY;
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    float x[32];
-                    scores(p, x);
-                    float top4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                    for (int j = 4; j < 32; ++j) top4[j & 3] = fmaxf(top4[j & 3], x[j]);
-                    top = fmaxf(top, fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])));
-                }
-                top *= mul;
+                // part 0 against the point so far, which is right but for the first steps
+                scores(0, x);
+                float top = most(x);
+                exponentials(x);
+                scores(1, x);
+                top = fmaxf(top, most(x)) * mul;
                 if (pair_any(quad, top > m + kAttnSlack || bad)) {
                     // rounded up: any point at or just above the maximum will do, and both threads take the same
                     const bf16 mine = __float2bfloat16_ru(top);
@@ -928,35 +956,15 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                         }
                         tmem_st_wait();
                     }
+                    sum0 = sum1 = 0ull;
+                    scores(0, x);
+                    exponentials(x);
+                    scores(1, x);
                 }
             }
-            const float ref = m == -INFINITY ? 0.f : m;
-            const uint64_t mul_2 = pack2(mul, mul), ref_2 = pack2(-ref, -ref);
-            uint64_t sum0 = 0ull, sum1 = 0ull;
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                uint32_t pk[16];
-                if (work) {
-                    float x[32];
-                    scores(p, x);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        float e0, e1;
-                        unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), mul_2, ref_2), e0, e1);
-                        e0 = exp2_fast(e0);
-                        e1 = exp2_fast(e1);
-                        if (j & 1) sum1 = add2(sum1, pack2(e0, e1));
-                        else sum0 = add2(sum0, pack2(e0, e1));
-                        pk[j] = pack_bf16x2(e0, e1);            // rounded for the tensor cores, summed as they are
-                    }
-                    tmem_st16(tmem + lanes + p * 64 + half * 32, pk);   // over scores that only this warp reads, and has read
-                    tmem_st_wait();
-                }
-                tc_fence_before();
-                if (!whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * p);        // a barrier for each part: a warp may be done with both before others with one
-            }
+            hand_over(0);
+            if (work) exponentials(x);
+            hand_over(1);
             float s0, s1;
             unpack2(add2(sum0, sum1), s0, s1);
             l += s0 + s1;
