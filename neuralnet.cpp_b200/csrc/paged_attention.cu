@@ -1281,13 +1281,21 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
     const long long pre = static_cast<long long>(prefix_stride) * kv.page_size, own = static_cast<long long>(table_stride) * kv.page_size;
     const long long pre_units = static_cast<long long>(groups) * kv.kv_heads * p.row_tiles, own_units = static_cast<long long>(groups) * size * kv.kv_heads * p.own_tiles;
-    // cached rows for a block when the tables are full: enough blocks for the machine a few times over, at least two steps each
-    const long long blocks = 148LL * 8;
-    long long chunk = ceil_div((p.tc ? 0 : pre_units * pre) + own_units * own, blocks);
-    chunk = std::min<long long>(std::max<long long>(ceil_div(chunk, 64) * 64, 128), 1 << 20);
+    // Rows of a run that a block takes when the tables are full.  Fewer make more partial results to write and join, more leave
+    // SMs idle behind the last ones (us, eight beams of 12 fp32 heads behind 901 rows: 64 rows 9.0, 128 10.5, 256 13.9, but behind
+    // 2000, where 64 are more than two blocks an SM, 14.5, 11.3, 14.7; two sequences of 32 bf16 heads behind 4000: 128 rows
+    // 15.2, 256 13.0; 64 queries of 16 heads behind 8192: 384 rows 41.5, 768 31.1, 2048 46).
+    const bool f32 = kv.dtype == 0;
+    const long long least = f32 ? (pre_units * ceil_div(pre, 64) <= 148 * 2 ? 64 : 128) : (p.rt <= 16 ? 256 : 128);
+    const long long share = ceil_div(ceil_div(pre_units * pre + own_units * own, 148LL * (f32 ? 4 : 6)), 64) * 64;
+    const long long chunk = std::min<long long>(std::max(share, least), 1 << 20);
     p.pre_splits = static_cast<int>(ceil_div(pre, chunk));
-    if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / std::max(pre_units, 1LL), 1), ceil_div(pre, 512)));
-    p.own_splits = static_cast<int>(ceil_div(own, chunk));
+    if (p.tc) p.pre_splits = static_cast<int>(std::min<long long>(std::max<long long>(148 * 2 / std::max(pre_units, 1LL), 1), ceil_div(pre, 256)));
+    // (tcgen05 tiles, one wave of blocks: 48 queries behind 901 rows, one head, 16.5 us with 256 rows a block at least, 22.9 with 512)
+    // own rows in bf16: 128 a warp, and four warps a task where there are that many (64 sequences of 16 heads with up to 512: 34.6 us
+    // with a warp for all of them, 31.5 with one for 128, 30.2 with a block; 128 sequences with up to 256: 41.0, 38.1, 39.4)
+    p.own_warps = f32 || own >= 512 ? 4 : 1;
+    p.own_splits = static_cast<int>(ceil_div(own, f32 ? chunk : 128 * p.own_warps));
     // a prefix and own rows of 128 at most: a block for both, without the join, takes 5.4 us where prefix, own rows and join take 7.6
     // (four beams of six heads behind 41 rows; behind 200 it would be 10.5 and 7.9)
     p.direct = !p.tc && pre > 0 && own > 0 && pre + own <= 128 && static_cast<long long>(groups) * size * kv.kv_heads <= 4 * 148;
@@ -1297,7 +1305,7 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
         p.pre_splits = 0;
         p.own_splits = 1;
     }
-    p.own_warps = kv.dtype == 0 || p.direct || ceil_div(own, std::max(1, p.own_splits)) > 512 ? 4 : 1;
+    if (p.direct) p.own_warps = 4;
     return p;
 }
 
