@@ -13,6 +13,9 @@
 // bound are looked at again.  (Comparing each logit with a running threshold on the way took 2000 of a tile's 3800 clocks: with
 // 1000 logits a warp and tile somebody always has one.)  The second kernel, already resident when the first ends, joins the spans'
 // sums and picks from the rows' lists.
+// 64 groups of 8 beams over 32768 bf16 logits, 16 continuations: 21.4 us, of which the picking is 6 and the reading about 12 (a tile of
+// 4096 takes a block 1400 clocks beside three others; its exponentials alone, at 16 an SM and clock, take 1024 of them).  One group
+// of 4 beams over 4096: 7.0 us, two launches of a few dependent steps.
 #include <algorithm>
 
 #include "common.cuh"

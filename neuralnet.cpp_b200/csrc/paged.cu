@@ -6,7 +6,9 @@ namespace nnb {
 // ---------------------------------------------------------------- append
 // For each new token: k, q rotated to the token's position, k and v rounded once to the cache's type and stored at the
 // token's row of its sequence's pages, q to q_out.  x[j] <- x[j] c - x[j+h/2] s, x[j+h/2] <- x[j+h/2] c + x[j] s, as rope_apply.
-// A thread takes VEC columns of one head's first half and the same columns of the second half.
+// A thread takes VEC columns of one head's first half and the same columns of the second half, 16 bytes of the narrower type at a
+// time where alignment allows.  Bound by memory where there is work: 8192 tokens of 16 heads of 64, fp32 into bf16, 28.2 us, 5400
+// GB/s; eight tokens of 12 heads take 2.0 us, a launch.
 struct AppendArgs {
     const void *q, *k, *v;
     void* q_out;
@@ -103,7 +105,9 @@ static int append_t(const nnb200_paged_kv& kv, int layer, const AppendArgs& a, c
 // ---------------------------------------------------------------- reorder
 // The state of slot b becomes that of its parent p: whole pages, which nobody writes any more, by copying table entries; the
 // page that is partly filled, which both slots will go on writing, by copying its rows into the slot's spare page.  Everything
-// is read from the old tables and written to new ones and to pages that no old table names, so no order matters.
+// is read from the old tables and written to new ones and to pages that no old table names, so no order matters.  A block per
+// slot and layer.  Bound by memory: 192 slots of 16 layers of 8 bf16 heads of 128, 30 rows of a page of 32 each, 113 us, 6700 GB/s
+// of reads and writes (755 MB); eight slots of 12 layers take 6.2 us, a launch and one trip to memory.
 struct ReorderArgs {
     const int *parent, *len, *table, *spare;
     int *len_out, *table_out, *spare_out;

@@ -126,9 +126,11 @@ __device__ __forceinline__ int far_of(const PagedAttnArgs& a, int shift, const A
 // 64 cached rows a step, a ring of STAGES steps filled by 16-byte asynchronous copies; WM warps take 16 query rows each, the
 // 4 / WM warps of a set of rows take turns at the step's cached rows and are joined at the end.  Cached rows that do not
 // exist are zero in shared memory (what lies there may be anything, and zero times it must be zero) and -inf as scores.
+// Bound by the chain of a step: 64 rows of 16 heads of 64 behind 8192 cached rows (34 MB, 5 us of memory's) take 26 us with launch
+// and join, one block an SM; more blocks with shorter runs leave more to join than they gain.
 template <int DP> struct AttnTile {
     static constexpr int KT = 64, CPR = DP / 8;                // cached rows a step, 16-byte chunks a row
-    static constexpr int STAGES = DP <= 64 ? 4 : (DP == 128 ? 3 : 2);
+    static constexpr int STAGES = DP <= 64 ? 4 : 2;
     static constexpr int BYTES = KT * DP * 2;
     static constexpr int SMEM = STAGES * 2 * BYTES + STAGES * (KT + 16) + 64;
     // chunk c of row r: eight rows of one chunk column fall into eight different 16-byte banks
@@ -388,6 +390,8 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
 // A lane looks up one cached row of a step, a step before it is copied; the copies get it by shuffle.  Rows in shared memory
 // are 16 bytes longer than they are: eight neighbours at one column meet no bank twice.  The reference point of the exponentials
 // moves only when a score is more than 2^8 above it: scores then need no maximum across lanes.
+// Bound by memory, behind 7 us of launch, first rows and join: 16 prefixes of 2047 rows, 16 heads of 64, eight queries each, 134 MB,
+// 27.5 us in all; 96 sequences' own rows, up to 1024, 8 heads of 128, 190 MB, 39 us.
 template <int DP> struct AttnStream {
     static constexpr int KW = DP <= 32 ? 32 : 16, ST = DP <= 64 ? 3 : 2, PITCH = DP * 2 + 16, CPR = DP / 8;
     static constexpr int PLANE = KW * PITCH, STAGE = 2 * PLANE, RING = ST * STAGE;
@@ -857,6 +861,8 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
             const int t0 = k.begin + i * KT;
             const bool whole = !gaps && t0 + KT <= k.end;
             uint32_t there[2] = {0xffffffffu, 0xffffffffu};
+            // before all else: it also says that the step before has used its V, whose place this step's takes
+            bad |= !wait_all(s_full, i, 11);
             if (!whole) {
                 // rows [from, from + count) of the step are this lane's, as bits of its 128
                 const int from = lane * high, count = box_of(i) < 0 ? 0 : min(high, k.end - (t0 + from));
@@ -875,7 +881,6 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                     if (!(wd >> (r & 31) & 1u)) *reinterpret_cast<uint4*>(sV + st * Tc::TILE + (idx >> 3) / KT * Tc::SUB + r * 128 + (idx & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
-            bad |= !wait_all(s_full, i, 11);
             // 32 scores of part p (cached rows [64 p, 64 p + 64) of the step), biased and masked
             auto scores = [&](int p, float (&x)[32]) {
                 uint32_t r[32];
@@ -1036,7 +1041,7 @@ int paged_attn_device_error(int* code)
 // 16-byte reads meet no bank twice.  fp32 products and sums throughout: infinities and NaN behave as in the formula, which
 // splitting a number into parts for the tensor cores would not keep.  With few rows a step is a chain of dependent
 // instructions: eight warps and a fixed RT, instead of four that count rows, took 13.5 us to 10.9 for eight beams of 12 heads
-// behind 901 rows.
+// behind 901 rows (9.2 since the join and the runs were changed).
 constexpr int kF32Threads = 256;
 template <int DP, int RT> struct AttnTile32 {
     static constexpr int KT = DP <= 64 ? 64 : 4096 / DP, LD = DP + 4, CPR = DP / 4, STAGES = 2;
@@ -1203,7 +1208,9 @@ __global__ void __launch_bounds__(kF32Threads) paged_attn_f32_kernel(PagedPool<f
 }
 
 // ---------------------------------------------------------------- the join
-// A block per query row: groups of dk / 4 threads take the slots in turn.
+// A block per query row: groups of dk / 4 threads take the slots in turn.  A few latencies of L2 and no work to speak of: about 2 us
+// behind the last block of the kernel in front, 6 us for 3072 rows of 128 columns and 13 places (20 MB) because 2368 blocks are
+// resident at a time.  Loading the first places before their maximum is known took 0.8 us out.
 template <typename T>
 __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int dk)
 {
@@ -1270,9 +1277,10 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     AttnPlan p;
     const int m = heads / kv.kv_heads;
     const long long rows = static_cast<long long>(size) * m;
-    // bf16: warps stream up to 16 query rows; beyond that mma.sync tiles take 32 or 64 of heads up to 64 wide and the tcgen05
-    // tiles 128 of wider ones, or more of them (us, tcgen05 | mma.sync, heads of 64 behind 8192 rows and own ones: 20 rows 31 | 27.5,
-    // 64 rows 36 | 35; heads of 128 behind 32768: 32 rows 49 | 72, 64 rows 52 | 87); heads over 128 have only mma.sync tiles
+    // bf16: warps stream up to 16 query rows; beyond that mma.sync tiles take up to 64 of heads up to 64 wide, and the tcgen05 tiles
+    // all of wider ones and more than 64 (us, tcgen05 | mma.sync, heads of 64 behind 8192 rows and own ones: 20 rows 27.2 | 21.5,
+    // 64 rows 36.5 | 31.0; heads of 128 behind 32768: 32 rows 44.5, 64 rows 46.7, where mma.sync tiles took 72 and 87, and 17 rows
+    // of them 43.7 where the stream takes 47.0 for 16); heads over 128 have only mma.sync tiles
     p.tc = kv.dtype == 1 && rows > (kv.head_dim <= 64 ? 64 : 16) && kv.head_dim <= 128 && prefix_stride > 0;
     const int few = std::max<long long>(prefix_stride > 0 ? rows : 0, m) <= 4 ? 4 : (std::max<long long>(prefix_stride > 0 ? rows : 0, m) <= 8 ? 8 : 16);
     p.rt = kv.dtype == 0 ? few : (p.tc ? 128 : (rows <= 8 ? 8 : (rows <= 16 || prefix_stride == 0 ? 16 : (rows <= 32 && kv.head_dim <= 64 ? 32 : 64))));
@@ -1296,9 +1304,10 @@ static AttnPlan attn_plan(const nnb200_paged_kv& kv, int groups, int size, int h
     // with a warp for all of them, 31.5 with one for 128, 30.2 with a block; 128 sequences with up to 256: 41.0, 38.1, 39.4)
     p.own_warps = f32 || own >= 512 ? 4 : 1;
     p.own_splits = static_cast<int>(ceil_div(own, f32 ? chunk : 128 * p.own_warps));
-    // a prefix and own rows of 128 at most: a block for both, without the join, takes 5.4 us where prefix, own rows and join take 7.6
-    // (four beams of six heads behind 41 rows; behind 200 it would be 10.5 and 7.9)
-    p.direct = !p.tc && pre > 0 && own > 0 && pre + own <= 128 && static_cast<long long>(groups) * size * kv.kv_heads <= 4 * 148;
+    // a block for a short prefix and the own rows behind it, without the join (us against the three launches' work in two, four beams of
+    // six heads: bf16 behind 41 rows 3.6 | 5.0, 200 rows 5.9 | 6.6; fp32, whose scores and values are plain products, behind 41 rows
+    // 5.6 | 5.5 with a launch less, 90 rows 7.3 | 5.7)
+    p.direct = !p.tc && pre > 0 && own > 0 && pre + own <= (f32 ? 64 : 256) && static_cast<long long>(groups) * size * kv.kv_heads <= 4 * 148;
     if (p.direct) {
         p.rt = p.own_rows = kv.dtype == 0 && m <= 4 ? 4 : (m <= 8 ? 8 : 16);
         p.own_tiles = static_cast<int>(ceil_div(m, p.own_rows));
@@ -1368,7 +1377,7 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
             }
             else {
                 const bool wide = p.own_rows == 16;
-                constexpr int both = std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));
+                constexpr int both = DP == 128 ? 0 : std::max(AttnTile<DP>::SMEM, AttnStream<DP>::smem(4));
                 if constexpr (DP != 128) if (p.rt == 64) return wide ? go(paged_attn_bf16_kernel<DP, 4, 2>, both, once[2]) : go(paged_attn_bf16_kernel<DP, 4, 1>, both, once[3]);
                 if constexpr (DP <= 64) if (p.rt == 32) return wide ? go(paged_attn_bf16_kernel<DP, 2, 2>, both, once[4]) : go(paged_attn_bf16_kernel<DP, 2, 1>, both, once[5]);
                 return wide ? go(paged_attn_bf16_kernel<DP, 1, 2>, AttnStream<DP>::smem(4), once[0]) : go(paged_attn_bf16_kernel<DP, 1, 1>, AttnStream<DP>::smem(4), once[1]);

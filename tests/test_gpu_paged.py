@@ -235,6 +235,14 @@ def test_attention_many_rows(g, heads, hk, dk, page, size, alibi):
     _check_attention(g, 1, heads, hk, dk, page, 2, size, prefix, own, alibi, seed=size, change=change)
 
 
+@pytest.mark.parametrize("heads,hk,dk,size", [(24, 12, 80, 20), (12, 12, 128, 17), (12, 12, 64, 70)])
+def test_attention_of_some_rows_behind_runs_of_several_steps(g, heads, hk, dk, size):
+    """Tiles that are not full of queries, runs of several steps that end inside one."""
+    own = [(5 * i) % 9 for i in range(size)]
+    _check_attention(g, 1, heads, hk, dk, 64, 1, size, [12358], own, seed=size)
+    _check_attention(g, 1, heads, hk, dk, 16, 1, size, [9001], own, alibi=1, seed=size)
+
+
 def test_attention_of_many_rows_large_scores_and_status_word(g):
     _check_attention(g, 1, 4, 4, 64, 16, 1, 100, [1500], [(7 * i) % 50 for i in range(100)], seed=9, spread=60.0)
     _check_attention(g, 1, 8, 2, 128, 32, 1, 30, [1500], [(7 * i) % 50 for i in range(30)], seed=9, spread=60.0)
@@ -329,6 +337,14 @@ def test_attention_short_contexts(g, dtype, heads, hk, dk, page, alibi):
         ptab[0, 0], otab[1, 0] = -1, kp.shape[0]
         return q, kp, vp, ptab, otab, plen, olen
     _check_attention(g, dtype, heads, hk, dk, page, 1, 2, [40], [9, 30], alibi, seed=2, change=change)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("heads,hk,dk,page", [(6, 6, 64, 16), (8, 2, 128, 8), (3, 1, 40, 8), (40, 2, 32, 16), (2, 2, 256, 8)])
+@pytest.mark.parametrize("prefix,own", [([33, 0, 1], [15, 0, -1, 1, 16, 2]), ([170, 9, 128], [1, 33, -1, 0, 64, 49])])
+def test_attention_short_prefixes_and_own_rows(g, dtype, heads, hk, dk, page, prefix, own):
+    _check_attention(g, dtype, heads, hk, dk, page, 3, 2, prefix, own, seed=3)
+    _check_attention(g, dtype, heads, hk, dk, page, 3, 2, prefix, own, alibi=1, seed=4, ld_extra=3)
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
