@@ -126,11 +126,12 @@ __device__ __forceinline__ int far_of(const PagedAttnArgs& a, int shift, const A
 // 64 cached rows a step, a ring of STAGES steps filled by 16-byte asynchronous copies; WM warps take 16 query rows each, the
 // 4 / WM warps of a set of rows take turns at the step's cached rows and are joined at the end.  Cached rows that do not
 // exist are zero in shared memory (what lies there may be anything, and zero times it must be zero) and -inf as scores.
-// Bound by the chain of a step: 64 rows of 16 heads of 64 behind 8192 cached rows (34 MB, 5 us of memory's) take 26 us with launch
-// and join, one block an SM; more blocks with shorter runs leave more to join than they gain.
+// Bound by the chain of a step: 64 rows of 16 heads of 64 behind 8192 cached rows (34 MB, 5 us of memory's) take 24.7 us with launch
+// and join, one block an SM; more blocks with shorter runs leave more to join than they gain.  Three stages instead of four leave
+// room for a fourth block of own rows: 20 queries with up to 512 rows each behind the same 21.4 us to 18.6.
 template <int DP> struct AttnTile {
     static constexpr int KT = 64, CPR = DP / 8;                // cached rows a step, 16-byte chunks a row
-    static constexpr int STAGES = DP <= 64 ? 4 : 2;
+    static constexpr int STAGES = DP <= 64 ? 3 : 2;
     static constexpr int BYTES = KT * DP * 2;
     static constexpr int SMEM = STAGES * 2 * BYTES + STAGES * (KT + 16) + 64;
     // chunk c of row r: eight rows of one chunk column fall into eight different 16-byte banks

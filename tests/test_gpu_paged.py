@@ -235,12 +235,12 @@ def test_attention_many_rows(g, heads, hk, dk, page, size, alibi):
     _check_attention(g, 1, heads, hk, dk, page, 2, size, prefix, own, alibi, seed=size, change=change)
 
 
-@pytest.mark.parametrize("heads,hk,dk,size", [(24, 12, 80, 20), (12, 12, 128, 17), (12, 12, 64, 70)])
+@pytest.mark.parametrize("heads,hk,dk,size", [(24, 12, 80, 20), (12, 12, 128, 17), (12, 12, 64, 66)])
 def test_attention_of_some_rows_behind_runs_of_several_steps(g, heads, hk, dk, size):
     """Tiles that are not full of queries, runs of several steps that end inside one."""
     own = [(5 * i) % 9 for i in range(size)]
-    _check_attention(g, 1, heads, hk, dk, 64, 1, size, [12358], own, seed=size)
-    _check_attention(g, 1, heads, hk, dk, 16, 1, size, [9001], own, alibi=1, seed=size)
+    _check_attention(g, 1, heads, hk, dk, 64, 1, size, [6300], own, seed=size)
+    _check_attention(g, 1, heads, hk, dk, 16, 1, size, [7003], own, alibi=1, seed=size)
 
 
 def test_attention_of_many_rows_large_scores_and_status_word(g):
