@@ -1210,18 +1210,19 @@ __global__ void __launch_bounds__(kF32Threads) paged_attn_f32_kernel(PagedPool<f
 
 // ---------------------------------------------------------------- the join
 // A block per query row: groups of dk / 4 threads take the slots in turn.  A few latencies of L2 and no work to speak of: about 2 us
-// behind the last block of the kernel in front, 6 us for 3072 rows of 128 columns and 13 places (20 MB) because 2368 blocks are
-// resident at a time.  Loading the first places before their maximum is known took 0.8 us out.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int dk)
+// behind the last block of the kernel in front, 6 us for 3072 rows of 128 columns and 13 places (20 MB) because not all blocks are
+// resident at a time.  Loading the first places before their maximum is known took 0.8 us out.  Blocks of 64 threads where rows are
+// many and narrow: 64 groups of eight behind 300 rows, 16 heads of 64, 75.9 us to 72.1 in all; of 128 columns no difference.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int dk)
 {
-    __shared__ float sx[128 * 4], sl[128], red[32];
+    __shared__ float sx[NT * 4], sl[NT], red[32];
     const long long row = blockIdx.x;
     int h = static_cast<int>(blockIdx.x);
     const int seq = a.by_heads.split(h), slots = a.slots;
     const bool live = sees(a, seq);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int vecs = dk / 4, sets = a.by_vecs.div(128), set = a.by_vecs.div(threadIdx.x), c = (threadIdx.x - set * vecs) * 4;
+    const int vecs = dk / 4, sets = a.by_vecs.div(NT), set = a.by_vecs.div(threadIdx.x), c = (threadIdx.x - set * vecs) * 4;
     const float2* st = a.stat + row * slots;
     const float* part = a.part + row * slots * dk + c;
     // a thread's first places are under way before their maximum is known
@@ -1238,7 +1239,7 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) m = fmaxf(m, s[u].x);
-    for (int i = AHEAD * sets + threadIdx.x; i < slots; i += 128) m = fmaxf(m, st[i].x);
+    for (int i = AHEAD * sets + threadIdx.x; i < slots; i += NT) m = fmaxf(m, st[i].x);
     m = block_max(m, red);
     const float ref = m == -INFINITY ? 0.f : m;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1403,7 +1404,8 @@ static int attention_t(const nnb200_paged_kv& kv, int layer, PagedAttnArgs a, co
         }
     }
     if (a.slots == 1) return 0;
-    NNB_TRY(launch_behind(paged_attn_join_kernel<T>, static_cast<unsigned>(rows), 128, 0, blocks > 0, s, a, kv.head_dim));
+    if (rows > 148 * 16 && kv.head_dim <= 64) NNB_TRY(launch_behind(paged_attn_join_kernel<T, 64>, static_cast<unsigned>(rows), 64, 0, blocks > 0, s, a, kv.head_dim));
+    else NNB_TRY(launch_behind(paged_attn_join_kernel<T, 128>, static_cast<unsigned>(rows), 128, 0, blocks > 0, s, a, kv.head_dim));
     return 0;
 }
 

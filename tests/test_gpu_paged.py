@@ -243,6 +243,13 @@ def test_attention_of_some_rows_behind_runs_of_several_steps(g, heads, hk, dk, s
     _check_attention(g, 1, heads, hk, dk, 16, 1, size, [7003], own, alibi=1, seed=size)
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("heads,hk,dk,groups,size", [(16, 16, 40, 3, 50), (40, 2, 32, 2, 33)])
+def test_attention_of_more_query_rows_than_are_joined_at_a_time(g, dtype, heads, hk, dk, groups, size):
+    own = [(13 * i) % 150 - 1 for i in range(groups * size)]
+    _check_attention(g, dtype, heads, hk, dk, 16, groups, size, [300, 0, 77][:groups], own, seed=heads)
+
+
 def test_attention_of_many_rows_large_scores_and_status_word(g):
     _check_attention(g, 1, 4, 4, 64, 16, 1, 100, [1500], [(7 * i) % 50 for i in range(100)], seed=9, spread=60.0)
     _check_attention(g, 1, 8, 2, 128, 32, 1, 30, [1500], [(7 * i) % 50 for i in range(30)], seed=9, spread=60.0)
