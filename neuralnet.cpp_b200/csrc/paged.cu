@@ -7,7 +7,7 @@ namespace nnb {
 // For each new token: k, q rotated to the token's position, k and v rounded once to the cache's type and stored at the
 // token's row of its sequence's pages, q to q_out.  x[j] <- x[j] c - x[j+h/2] s, x[j+h/2] <- x[j+h/2] c + x[j] s, as rope_apply.
 // A thread takes VEC columns of one head's first half and the same columns of the second half, 16 bytes of the narrower type at a
-// time where alignment allows.  Bound by memory where there is work: 8192 tokens of 16 heads of 64, fp32 into bf16, 28.2 us, 5400
+// time where alignment allows.  Bound by memory where there is work: 8192 tokens of 16 heads of 64, fp32 into bf16, 27.8 us, 5450
 // GB/s; eight tokens of 12 heads take 2.0 us, a launch.
 struct AppendArgs {
     const void *q, *k, *v;
@@ -55,19 +55,19 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedPool<T> pool, Ap
     for (long long w = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; w < items; w += static_cast<long long>(gridDim.x) * blockDim.x) {
         const int tok = static_cast<int>(w / per_token), r = static_cast<int>(w - static_cast<long long>(tok) * per_token);
         const int part = r / vph, j = (r - part * vph) * VEC;
-        const int seq = a.seq_of ? a.seq_of[tok] : tok, row = a.row_of[tok];
-        if (seq < 0 || seq >= a.seqs || row < 0 || (row >> pool.page_shift) >= a.table_stride) continue;
-        const int page = a.table[static_cast<long long>(seq) * a.table_stride + (row >> pool.page_shift)];
-        const int pos = a.rope_pos ? a.rope_pos[tok] : row;
-        if (page < 0 || page >= pool.pages || (a.rope && (pos < 0 || pos >= a.rope_len))) continue;
         const bool is_q = part < a.heads, is_k = !is_q && part < a.heads + pool.kv_heads;
         if (is_q && !a.q) continue;
         const int h = is_q ? part : (is_k ? part - a.heads : part - a.heads - pool.kv_heads);
         const TS* src = is_q ? static_cast<const TS*>(a.q) + tok * a.ldq : static_cast<const TS*>(is_k ? a.k : a.v) + tok * a.ldkv;
         src += static_cast<long long>(h) * pool.dk + j;
-        float lo[VEC], hi[VEC];
+        float lo[VEC], hi[VEC];                                 // on their way while the row's place is looked up
         load_vec<TS, VEC>(src, lo);
         load_vec<TS, VEC>(src + half, hi);
+        const int seq = a.seq_of ? a.seq_of[tok] : tok, row = a.row_of[tok];
+        if (seq < 0 || seq >= a.seqs || row < 0 || (row >> pool.page_shift) >= a.table_stride) continue;
+        const int page = a.table[static_cast<long long>(seq) * a.table_stride + (row >> pool.page_shift)];
+        const int pos = a.rope_pos ? a.rope_pos[tok] : row;
+        if (page < 0 || page >= pool.pages || (a.rope && (pos < 0 || pos >= a.rope_len))) continue;
         if (a.rope && (is_q || is_k)) {
             const float* cs = a.rope + static_cast<long long>(pos) * half + j;
             const float* sn = cs + static_cast<long long>(a.rope_len) * half;
@@ -105,9 +105,10 @@ static int append_t(const nnb200_paged_kv& kv, int layer, const AppendArgs& a, c
 // ---------------------------------------------------------------- reorder
 // The state of slot b becomes that of its parent p: whole pages, which nobody writes any more, by copying table entries; the
 // page that is partly filled, which both slots will go on writing, by copying its rows into the slot's spare page.  Everything
-// is read from the old tables and written to new ones and to pages that no old table names, so no order matters.  A block per
-// slot and layer.  Bound by memory: 192 slots of 16 layers of 8 bf16 heads of 128, 30 rows of a page of 32 each, 113 us, 6700 GB/s
-// of reads and writes (755 MB); eight slots of 12 layers take 6.2 us, a launch and one trip to memory.
+// is read from the old tables and written to new ones and to pages that no old table names, so no order matters.  A block each
+// for a slot's and layer's keys and values.  Bound by memory: 192 slots of 16 layers of 8 bf16 heads of 128, 30 rows of a page of 32 each, 104 us, 755 MB read and written
+// (parents that several slots share are read from L2); eight slots of 12 layers 4.1 us, a launch and a few trips to memory.  With keys
+// and values in one block and a vector at a time they took 113 and 6.1 us.
 struct ReorderArgs {
     const int *parent, *len, *table, *spare;
     int *len_out, *table_out, *spare_out;
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(PagedPool<T> pool, lo
     const int* from = a.table + static_cast<long long>(p) * a.table_stride;
     const int* mine = a.table + static_cast<long long>(slot) * a.table_stride;
     const int spare = a.spare[slot];
-    if (layer == 0) {
+    if (layer == 0 && blockIdx.z == 0) {
         int* to = a.table_out + static_cast<long long>(slot) * a.table_stride;
         for (int j = threadIdx.x; j < a.table_stride; j += blockDim.x) to[j] = j < full ? from[j] : (j == full && rest ? spare : mine[j]);
         if (threadIdx.x == 0) {
@@ -139,17 +140,27 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(PagedPool<T> pool, lo
     if (src < 0 || src >= pool.pages || spare < 0 || spare >= pool.pages || src == spare) return;
     constexpr int N = Vec16<T>::N;
     const int per_head = rest * pool.dk / N, all = per_head * pool.kv_heads;       // head_dim is a whole number of 16-byte vectors
-    for (int w = threadIdx.x; w < 2 * all; w += blockDim.x) {
-        T* pages = (w < all ? pool.k : pool.v) + layer * layer_stride;
-        const int i = w < all ? w : w - all, h = i / per_head, e = (i - h * per_head) * N;
-        st16(pages + pool.at(spare, h, 0) + e, ld16(pages + pool.at(src, h, 0) + e));
+    constexpr int U = 4;                                        // vectors of a thread on their way at a time
+    T* const pages = (blockIdx.z == 0 ? pool.k : pool.v) + layer * layer_stride;
+    for (int w0 = threadIdx.x; w0 < all; w0 += U * blockDim.x) {
+        Vec16<T> v[U];
+        T* to[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = w0 + u * blockDim.x, h = i / per_head, e = (i - h * per_head) * N;
+            if (i >= all) { to[u] = nullptr; continue; }
+            to[u] = pages + pool.at(spare, h, 0) + e;
+            v[u] = ld16(pages + pool.at(src, h, 0) + e);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) if (to[u]) st16(to[u], v[u]);
     }
 }
 
 template <typename T>
 static int reorder_t(const nnb200_paged_kv& kv, int slots, const ReorderArgs& a, cudaStream_t s)
 {
-    beam_reorder_kernel<T><<<dim3(static_cast<unsigned>(slots), static_cast<unsigned>(kv.layers)), 256, 0, s>>>(paged_pool<T>(kv, 0), kv.layer_stride, a);
+    beam_reorder_kernel<T><<<dim3(static_cast<unsigned>(slots), static_cast<unsigned>(kv.layers), 2), 256, 0, s>>>(paged_pool<T>(kv, 0), kv.layer_stride, a);
     NNB_LAUNCH_CHECK();
     return 0;
 }

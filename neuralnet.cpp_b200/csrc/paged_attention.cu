@@ -1210,8 +1210,8 @@ __global__ void __launch_bounds__(kF32Threads) paged_attn_f32_kernel(PagedPool<f
 
 // ---------------------------------------------------------------- the join
 // A block per query row: groups of dk / 4 threads take the slots in turn.  A few latencies of L2 and no work to speak of: about 2 us
-// behind the last block of the kernel in front, 6 us for 3072 rows of 128 columns and 13 places (20 MB) because not all blocks are
-// resident at a time.  Loading the first places before their maximum is known took 0.8 us out.  Blocks of 64 threads where rows are
+// behind the last block of the kernel in front, 6 us for 96 queries of 32 heads of 128 and 13 places (20 MB) because not all blocks
+// are resident at a time.  Loading the first places before their maximum is known took 0.8 us out.  Blocks of 64 threads where rows are
 // many and narrow: 64 groups of eight behind 300 rows, 16 heads of 64, 75.9 us to 72.1 in all; of 128 columns no difference.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a, int dk)
