@@ -690,8 +690,8 @@ template <int DP> struct AttnTc {
     static constexpr int NS = DP / 64, ST = DP == 64 ? 2 : 1, KT = 128;
     static constexpr int SUB = 128 * 128;                       // bytes of 128 rows by 64 columns
     static constexpr int TILE = NS * SUB;
-    static constexpr int OFF_K = TILE, OFF_V = OFF_K + ST * TILE, OFF_X = OFF_V + ST * TILE, OFF_BAR = OFF_X + 2 * 128 * 2;
-    static constexpr int TILES = OFF_BAR + 256;                 // DP = 128: two blocks fit an SM, with 256 bytes to spare
+    static constexpr int OFF_K = TILE, OFF_V = OFF_K + ST * TILE, OFF_X = OFF_V + ST * TILE, OFF_BAR = OFF_X + 2 * 128 * 4;
+    static constexpr int TILES = OFF_BAR + 256;                 // two blocks fit an SM: 97.3 KB each with DP = 128, 81.3 KB with 64
     static constexpr uint32_t TMEM_COLS = 256;                  // scores [0, 128), O [128, 128 + DP)
 };
 
@@ -715,7 +715,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     using Tc = AttnTc<DP>;
     constexpr int ST = Tc::ST, NS = Tc::NS, KT = Tc::KT;
     uint8_t *sQ = smem, *sK = smem + Tc::OFF_K, *sV = smem + Tc::OFF_V;
-    bf16* sX = reinterpret_cast<bf16*>(smem + Tc::OFF_X);       // (half, row)
+    float* sX = reinterpret_cast<float*>(smem + Tc::OFF_X);     // (half, row)
     float* sL = reinterpret_cast<float*>(sQ);                   // (half, row), once the query tile has been used
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tc::OFF_BAR);
     const uint32_t bar0 = smem_u32(bars);
@@ -941,11 +941,11 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                 scores(1, x);
                 top = fmaxf(top, most(x)) * mul;
                 if (pair_any(quad, top > m + kAttnSlack || bad)) {
-                    // rounded up: any point at or just above the maximum will do, and both threads take the same
-                    const bf16 mine = __float2bfloat16_ru(top);
-                    sX[half * 128 + row] = mine;
+                    // both threads take the same point, the maximum itself: one that is rounded up lies above large scores by more
+                    // than their exponentials can bear (a step of bf16 is 256 beyond 2^15)
+                    sX[half * 128 + row] = top;
                     if (pair_any(quad, bad)) { bad = true; break; }              // both warps leave here
-                    top = fmaxf(__bfloat162float(mine), __bfloat162float(sX[(half ^ 1) * 128 + row]));
+                    top = fmaxf(top, sX[(half ^ 1) * 128 + row]);
                     const bool move = top > m + kAttnSlack;
                     const float back = move ? exp2_fast(m - top) : 1.0f;          // 0 from -inf
                     if (move) m = top;

@@ -256,6 +256,34 @@ def test_attention_of_many_rows_large_scores_and_status_word(g):
     assert g.gemm_status() == 0
 
 
+@pytest.mark.parametrize("heads,hk,dk,size", [(2, 2, 64, 90), (4, 1, 128, 20), (2, 2, 64, 30), (2, 2, 64, 5)])
+@pytest.mark.parametrize("prefix,own", [([700], 21), ([200], 0)])
+def test_attention_scores_of_hundreds_of_thousands(g, heads, hk, dk, size, prefix, own):
+    """Scores of 2e4 to 7e5 of either sign, that differ by little: column 0 gives all of a query's scores one large number, the
+    others whole numbers.  Products and partial sums are whole numbers below 2^24, exact in fp32 in whatever order, so the
+    weights depend only on differences of tens, whose scaling is off by 2^-24 twice: the large number is the same in every one."""
+    import torch
+    n = size
+    q, kp, vp, ptab, otab, plen, olen = _attention_inputs(1, heads, hk, dk, 16, 1, size, prefix, [(7 * i) % (own + 1) for i in range(n)], dk + size)
+    r = np.random.default_rng(3)
+    kp = np.where(np.isnan(kp), kp, r.integers(-2, 3, kp.shape)).astype(np.float32)
+    q = r.integers(-2, 3, q.shape).astype(np.float32)
+    kp[..., 0] = np.where(np.isnan(kp[..., 0]), np.nan, 128.0)
+    q[..., 0] = 2.0 ** r.integers(11, 16, q.shape[:2]) * r.choice([-1.0, 1.0], q.shape[:2])
+    q[0, 0, 0], q[1, 0, 0] = 2.0 ** 15, -2.0 ** 15
+    kt, vt = torch.from_numpy(kp).cuda().bfloat16(), torch.from_numpy(vp).cuda().bfloat16()
+    want, want_lse, _, _ = ref.attention(q.astype(np.float64), _f64(kt), _f64(vt), ptab, plen, otab, olen, size, 0, 1)
+    size_v, _, _, _ = ref.attention(q.astype(np.float64), _f64(kt), np.abs(_f64(vt)), ptab, plen, otab, olen, size, 0, 1)
+    got, got_lse, _ = _attention(g, 1, q, kt, vt, ptab, plen, otab, olen, size, 0)
+    # differences of at most 2 * 4 * dk / sqrt(dk) * log2(e) in powers of two, rounded with the factor and with the sum; an exponential
+    # 4 steps, sums of `total` terms; the weight's and the result's rounding to bf16
+    total = prefix[0] + own
+    weight = 2 * (2 * 8 * np.sqrt(dk) * 1.45 * ref.U + 4 * ref.U) + 2 * (total + 40) * ref.U + ref.HALF_STEP[1]
+    assert np.all(np.abs(got - want) <= weight * size_v + ref.HALF_STEP[1] * np.abs(want) + 1e-37), float(np.abs(got - want).max())
+    assert np.all(np.abs(got_lse - want_lse) <= 6 * ref.U * np.abs(want_lse) + (total + 40) * ref.U + 1e-4)
+    assert g.gemm_status() == 0
+
+
 @pytest.mark.parametrize("heads,hk,dk,size", [(2, 2, 64, 80), (4, 1, 128, 40), (2, 2, 64, 30), (1, 1, 256, 20)])
 def test_attention_of_many_rows_meets_infinities(g, heads, hk, dk, size):
     """A key of -inf has no weight, a value of +inf is one column's, a NaN key everybody's that sees it."""
