@@ -2,8 +2,10 @@
 //   score_b + logit_bv - log sum_u exp(logit_bu),
 // the n best, best first; equal values go to the lower (b, v).
 // Which of two continuations is better decides what a program answers.  A score and a logit are exact and values are compared
-// in 64 bits; the normaliser, the only rounded part, is summed in 64 bits from exponentials in 32, off by less than 1.5e-6 of
-// one (ex2 2^-22, its argument 2^-24 of about 10 twice, six additions in 32 bits), most often by less than 1e-7.  Where
+// in 64 bits; the normaliser, the only rounded part, is summed in 64 bits from exponentials in 32, off by less than 2.3e-6, most
+// often by less than 1e-7.  An exponential of a distance d to the reference point is off by half a step of d and of
+// d log2(e), 2^-22 for ex2 and six additions of 2^-24.  No d is above kSelAhead: 1.2e-6 for those from -8 up, 1.8e-6 for -16 to
+// -8, 2.3e-6 for -22 to -16; all further below, 2.9e-6, is at most 2^31 e^-22 = 0.6 of the largest exponential.  Where
 // continuations of two beams come closer than that, which happens to one group in some hundreds, their beams' normalisers
 // are computed again in 64 bits, as sums of whole numbers: exact to 1e-12, and the same in whatever order a row holds its logits.
 //
@@ -30,6 +32,7 @@ constexpr int kSelMost = 128;                                   // continuations
 constexpr int kSelSlack = 256;                                  // a list this much longer than n is cut back to n
 constexpr int kSelList = kSelTile + kSelMost + kSelSlack;       // a tile may go into the list whole
 constexpr int kSelTiles = 16;                                   // tiles of a span at most
+constexpr float kSelAhead = 8.0f;                               // what a logit may be above the reference point of its exponential
 constexpr int kSelPieces = kSelList / kSelPer - 4;              // threads' shares of tiles that may go into the list together
 
 struct alignas(16) SpanSum { double sum; float ref; };          // of exponentials against the reference point
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(kSelThreads) select_scan_kernel(const __grid_c
 #pragma unroll
             for (int w = 0; w < kSelWarps; ++w) ref = fmaxf(ref, sh.ref[w]);
         }
-        if (top > ref + 64.0f) { sum *= ref == -INFINITY ? 0.0 : exp(static_cast<double>(ref) - top); ref = top; }
+        if (top > ref + kSelAhead) { sum *= ref == -INFINITY ? 0.0 : exp(static_cast<double>(ref) - top); ref = top; }
         const float r = ref == -INFINITY ? 0.f : -ref;
         const uint64_t minus_ref = pack2(r, r);
         float part[4];
@@ -313,7 +316,7 @@ __device__ __forceinline__ unsigned long long order_of(double x)
 __device__ __forceinline__ double value_of(unsigned long long order) { return __longlong_as_double(static_cast<long long>(order >> 63 ? order & ~(1ull << 63) : ~order)); }
 __device__ __forceinline__ bool better(const Cand& x, const Cand& y) { return x.key > y.key || (x.key == y.key && x.at < y.at); }
 constexpr int kPickList = 2048;
-constexpr double kNear = 4e-6;                                  // values of two beams this close are compared again, exactly
+constexpr double kNear = 5e-6;                                  // values of two beams this close are compared again, exactly: twice a normaliser's error
 
 template <int W> struct PickShared {
     double norm[64];            // log-sum-exp of each beam; NaN: its logits offer nothing

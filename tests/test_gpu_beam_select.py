@@ -155,3 +155,41 @@ def test_select_more_candidates_than_a_tile_of_a_long_row(g):
     second[:, 127] = 1.0
     logits[:, 0, 4096:] = second.reshape(-1)
     _check(g, 0, logits, np.zeros((groups, 1)), None, -1, n)
+
+
+def _exponential_error(v, ref_point):
+    """Error of exp(v - ref_point) where v - ref_point, and its product with log2(e) in two parts, are rounded to fp32: what
+    a reference point far below a logit costs."""
+    d = (v - ref_point).astype(np.float32)
+    hi, lo = np.float32(1.4426950216293335), np.float32(1.925963033500e-8)
+    x = (d.astype(np.float64) * np.float64(hi) + (d * lo).astype(np.float64)).astype(np.float32)
+    return np.exp2(x.astype(np.float64)) / np.exp(v.astype(np.float64) - ref_point.astype(np.float64)) - 1.0
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("gap", [60.0, 45.0, 25.0, 12.0, 7.0])
+def test_select_rows_whose_peak_lies_far_above_their_first_tile(g, dtype, gap):
+    """One logit `gap` above the first 4096, chosen so that 32 bits err upwards in one beam and downwards in the other, of
+    two whose best values are 2e-6 apart; rows of two tiles that one block reads."""
+    groups, vocab, half = 600, 8192, gap / 2
+    r = np.random.default_rng(int(gap))
+    logits = (-half - 9 + r.standard_normal((groups, 2, vocab))).clip(None, -half - 2).astype(np.float32)
+    first, peak = (-half + 0.9 * r.random(400000)).astype(np.float32), (half + 0.9 * r.random(400000)).astype(np.float32)
+    order = np.argsort(_exponential_error(peak, first))
+    for b, picked in ((0, order[-groups:]), (1, order[:groups])):
+        logits[:, b, 77], logits[np.arange(groups), b, 4096 + r.integers(0, 4096, groups)] = first[picked], peak[picked]
+    if dtype:
+        import torch
+        logits = torch.from_numpy(logits).bfloat16().float().numpy()
+    x = logits.astype(np.float64)
+    top = x.max(axis=2)
+    best = -np.log(np.exp(x - top[..., None]).sum(axis=2))                     # the best candidate of each beam
+    scores = np.zeros((groups, 2), np.float32)
+    scores[:, 1] = best[:, 0] - best[:, 1] - 2e-6
+    scores[::2, 1] += np.float32(4e-6)
+    want = ref.select(x, scores.astype(np.float64), None, -1, 4)
+    parent, token, score, _ = _run(g, dtype, logits, scores, None, -1, 4)
+    assert [[(r[0], r[1]) for r in row] for row in want] == [[(int(a), int(b)) for a, b in zip(p, t)] for p, t in zip(parent, token)]
+    w = np.array([[r[2] for r in row] for row in want])
+    # one rounding to fp32, and the normaliser's stated bound
+    assert np.all(np.abs(score - w) <= 2.0 ** -24 * np.abs(w) + 2.3e-6)
