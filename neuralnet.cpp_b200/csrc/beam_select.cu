@@ -7,7 +7,8 @@
 // d log2(e), 2^-22 for ex2 and six additions of 2^-24.  No d is above kSelAhead: 1.2e-6 for those from -8 up, 1.8e-6 for -16 to
 // -8, 2.3e-6 for -22 to -16; all further below, 2.9e-6, is at most 2^31 e^-22 = 0.6 of the largest exponential.  Where
 // continuations of two beams come closer than that, which happens to one group in some hundreds, their beams' normalisers
-// are computed again in 64 bits, as sums of whole numbers: exact to 1e-12, and the same in whatever order a row holds its logits.
+// are computed again in 64 bits, as sums of whole multiples of 2^-62: off by 2^-63 an exponential (5e-13 for 2^22 of them) and the
+// roundings of exp and log, and the same in whatever order a row holds its logits.
 //
 // Two kernels.  The first reads the logits once, bound by memory and the exponentials: a block per span of a row sums its
 // exponentials and keeps the maximum of each thread's share of each tile.  The order within a row does not depend on the
@@ -324,7 +325,8 @@ template <int W> struct PickShared {
     Cand list[kPickList], best[kSelMost];
     uint32_t sw[W][2];
     Cand red[W], last;
-    unsigned long long part[W], again;                  // again: beams whose normalisers have to be exact
+    ulonglong2 part[W];
+    unsigned long long again;                           // beams whose normalisers have to be exact
     int count, ended[64];
 };
 
@@ -339,27 +341,33 @@ __device__ __forceinline__ void put(const SelectArgs& a, const PickShared<W>& sh
     if (a.ended_out) a.ended_out[to] = !none && (sh.ended[c.beam] || token == a.eos) ? 1 : 0;
 }
 
-// log-sum-exp of a row whose sum is finite, by the whole block: exponentials in 64 bits, added as multiples of 2^-shift, 62 bits in all
+// log-sum-exp of a row whose sum is finite, by the whole block: exponentials in 64 bits, none above 1, added as multiples of 2^-62.  Their
+// upper and lower 31 bits are added apart (x: below 2^32 each, y: below 2^31), so that 2^31 of them fit.
 template <typename T, int W>
 __device__ double exact_norm(const SelectArgs& a, PickShared<W>& sh, int row)
 {
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, shift = 62 - (32 - __clz(a.vocab));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float m = -INFINITY;                                        // the first entry of a span is its maximum
     for (int i = 0; i < a.spans; ++i) { const int2 e = a.list[(static_cast<long long>(row) * a.spans + i) * a.n]; if (e.y >= 0) m = fmaxf(m, __int_as_float(e.x)); }
-    const double scale = static_cast<double>(1ull << shift);
-    unsigned long long sum = 0;
+    ulonglong2 sum = make_ulonglong2(0, 0);
+    auto add = [&sum](unsigned long long hi, unsigned long long lo) { sum.x += hi; sum.y += lo; };
 #pragma unroll 8
-    for (int i = threadIdx.x; i < a.vocab; i += (W * 32)) sum += __double2ull_rn(exp(static_cast<double>(to_f32(x[i])) - m) * scale);
+    for (int i = threadIdx.x; i < a.vocab; i += (W * 32)) {
+        const unsigned long long e = __double2ull_rn(exp(static_cast<double>(to_f32(x[i])) - m) * 0x1p62);
+        add(e >> 31, e & 0x7fffffffull);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 16; o > 0; o >>= 1) add(__shfl_xor_sync(0xffffffffu, sum.x, o), __shfl_xor_sync(0xffffffffu, sum.y, o));
     __syncthreads();
     if (lane == 0) sh.part[warp] = sum;
     __syncthreads();
-    sum = 0;
+    sum = make_ulonglong2(0, 0);
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum += sh.part[w];
-    return static_cast<double>(m) + log(static_cast<double>(sum) / scale);
+    for (int w = 0; w < W; ++w) add(sh.part[w].x, sh.part[w].y);
+    // the same whole number whatever the order: first the carry, then to 64 bits of floating point
+    sum.x += sum.y >> 31;
+    return static_cast<double>(m) + log(static_cast<double>(sum.x) * 0x1p-31 + static_cast<double>(sum.y & 0x7fffffffull) * 0x1p-62);
 }
 
 template <typename T, int W>

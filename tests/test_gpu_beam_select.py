@@ -193,3 +193,16 @@ def test_select_rows_whose_peak_lies_far_above_their_first_tile(g, dtype, gap):
     w = np.array([[r[2] for r in row] for row in want])
     # one rounding to fp32, and the normaliser's stated bound
     assert np.all(np.abs(score - w) <= 2.0 ** -24 * np.abs(w) + 2.3e-6)
+
+
+@pytest.mark.parametrize("log_vocab,fraction", [(22, 0.49), (22, -0.49), (20, 0.49)])
+def test_select_many_small_exponentials_in_close_candidates(g, log_vocab, fraction):
+    """A peak over 2^20 or 2^22 equal logits whose exponentials are 1.49 or 1.51 times 2^(log_vocab - 61), against a beam that has
+    only its peak: sums as multiples of that step would be off by half a step for each of them."""
+    vocab = 1 << log_vocab
+    logits = np.full((1, 2, vocab), -np.inf, dtype=np.float32)
+    term = (1.49 if fraction > 0 else 1.51) * 2.0 ** (log_vocab - 61)
+    logits[0, 0], logits[0, :, 1000] = np.log(term), 0.0
+    off = vocab * 0.49 * 2.0 ** (log_vocab - 61)
+    best = -np.log1p((vocab - 1) * np.exp(np.float64(logits[0, 0, 0])))
+    _check(g, 0, logits, np.array([[0.0, best + (off if fraction > 0 else -off) / 2]]), None, -1, 2)
