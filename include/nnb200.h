@@ -503,8 +503,8 @@ int nnb200_paged_attention(const nnb200_paged_kv* kv, int layer, const void* q, 
  * group), token, scores_out and ended_out (may be NULL), each (groups, n).  A beam with ended[b] != 0 (NULL: none) has one continuation: the
  * token eos at its own score.  ended_out: the parent had ended, or the token is eos (-1: no such token).  -inf and NaN values
  * are no continuations, nor is anything of a row that holds NaN or +inf; places that nothing is left for get parent -1,
- * token -1, score -inf.  Up to 64 beams.  Values are compared in 64 bits; the normaliser is summed in 64 bits from
- * exponentials in 32. */
+ * token -1, score -inf.  Up to 64 beams, beams * vocab below 2^31, vocab below 2^31 - 2^16.  Values are compared in 64 bits;
+ * the normaliser is summed in 64 bits from exponentials in 32, off by less than 2.3e-6, and exact where that decides the order. */
 size_t nnb200_beam_select_scratch_bytes(int groups, int beams, int vocab, int n);
 int nnb200_beam_select(const void* logits, long long ld, int dtype, int groups, int beams, int vocab, const float* scores,
                        const int32_t* ended, int eos, int n, int32_t* parent, int32_t* token, float* scores_out, int32_t* ended_out,

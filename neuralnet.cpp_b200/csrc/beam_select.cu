@@ -568,6 +568,7 @@ static const char* select_shape_error(int groups, int beams, int vocab, int n)
     if (groups < 0) return "negative size";
     if (beams < 1 || beams > 64) return "beams must be from 1 to 64";
     if (vocab < 1 || static_cast<long long>(beams) * vocab > INT_MAX) return "vocab must be positive, and beams * vocab below 2^31";
+    if (vocab > INT_MAX - kSelTiles * kSelTile) return "vocab must be below 2^31 - 2^16";        // tokens are counted to the end of a row's last span
     if (n < 1 || n > kSelMost || n > static_cast<long long>(beams) * vocab) return "the number of continuations must be from 1 to 128, and at most beams * vocab";
     if (static_cast<long long>(groups) * beams > INT_MAX / 256) return "too many beams for one call";
     if (static_cast<long long>(beams) * select_spans(groups, beams, vocab) * n > INT_MAX / 2) return "too many candidates for one call";

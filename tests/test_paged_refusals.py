@@ -72,6 +72,15 @@ def test_select_refuses(change):
     refused("nnb200_beam_select", *select_args(**change))
 
 
+@pytest.mark.parametrize("vocab", [2 ** 31 - 1, 2 ** 31 - 2 ** 16])
+def test_select_refuses_vocabularies_whose_last_tile_ends_beyond_32_bits(vocab):
+    """A block reads spans of up to 2^16 logits and counts tokens in 32 bits to the end of the last one."""
+    assert nnb.lib.nnb200_beam_select_scratch_bytes(1, 1, vocab, 4) == 0
+    refused("nnb200_beam_select", *select_args(groups=1, beams=1, vocab=vocab, ld=vocab, n=4))
+    assert nnb.lib.nnb200_beam_select_scratch_bytes(1, 1, 2 ** 31 - 2 ** 16 - 1, 4) > 0
+    assert nnb.lib.nnb200_beam_select_scratch_bytes(1, 63, (2 ** 31 - 1) // 63, 4) > 0
+
+
 def reorder_args(kv_=None, **change):
     a = dict(groups=2, beams=3, parent=P, len=P, table=P, spare=P, len_out=2 * P, table_out=2 * P, spare_out=2 * P, stride=4, stream=None)
     a.update(change)
