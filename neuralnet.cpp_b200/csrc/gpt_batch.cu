@@ -117,7 +117,8 @@ static const char* batch_error(const nnb200_gpt_config* cfg, int seqs, int new_r
     if (dk % 8 || dk > 256) return "the head size must be a multiple of 8, up to 256";
     if (seqs < 1 || seqs > 1024) return "1 to 1024 sequences";
     if (new_rows < 1 || new_rows > cfg->seq) return "new rows: from 1 to seq";
-    // a layer's pages, counted in rows of a head, and the attention's queries (its own limits)
+    // a layer's pages, counted in rows of a head, and the attention's queries and heads (its own limits)
+    if (cfg->heads > 65535 || static_cast<long long>(seqs) * cfg->heads > INT_MAX / 512) return "too many heads for this many sequences";
     const long long pages = ceil_div(cfg->seq, kBatchPage) + static_cast<long long>(seqs) * (ceil_div(new_rows, kBatchPage) + 1);
     if (pages * cfg->heads * kBatchPage > INT_MAX || pages * (ceil_div(new_rows, kBatchPage) + 1) > INT_MAX) return "too many sequences for rows this long";
     return nullptr;

@@ -138,6 +138,14 @@ def test_batch_refuses_shapes(change, seqs, rows):
     refused("nnb200_gpt_batch_reorder", C.byref(c), P, seqs, rows, P, None)
 
 
+@pytest.mark.parametrize("heads,seqs", [(8192, 512), (70000, 1)])
+def test_batch_refuses_more_heads_than_its_attention_takes(heads, seqs):
+    """At once, and not in the first step behind a prompt."""
+    c = batch_cfg(d_model=8 * heads, heads=heads, layers=1)
+    assert nnb.lib.nnb200_gpt_batch_workspace_bytes(C.byref(c), seqs, 4) == -1
+    refused("nnb200_gpt_batch_begin", C.byref(c), P, P, seqs, 4, 10, None)
+
+
 def test_batch_refuses_arguments():
     c = batch_cfg()
     assert nnb.lib.nnb200_gpt_batch_workspace_bytes(C.byref(c), 4, 8) > 0
