@@ -682,8 +682,9 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
 // stood: with P in shared memory the products' operands, P and the arriving tiles asked for 3600 clocks of shared memory's
 // bandwidth a step of both blocks, of 4200 that it took, although the next step's S could then start half a P V earlier.  64 cached rows a step instead (an S of 128 x 64 takes the tensor core as long as one of 128 x 128) had the issue
 // of products as its bound: 2400 clocks for 64 rows and block, 12 products of 130 clocks.
-// Every wait is bounded; one that gives up raises a status word, the others see it, and the block drains: the two threads of a
-// row leave together, at the barrier where they compare notes.
+// Every wait is bounded; one that gives up raises a status word, the others see it, and the block drains: loads and products that
+// have been issued are waited for (again with a bound), and the two threads of a row leave together, at the barrier where they
+// compare notes.
 __device__ int g_paged_attn_error = 0;
 
 template <int DP> struct AttnTc {
@@ -720,8 +721,8 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tc::OFF_BAR);
     const uint32_t bar0 = smem_u32(bars);
     const uint32_t k_full = bar0, k_empty = bar0 + 8 * ST, v_full = bar0 + 16 * ST, v_empty = bar0 + 24 * ST, s_full = bar0 + 32 * ST,
-                   p_full = s_full + 8, pv_done = s_full + 24, q_full = s_full + 32;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * ST + 5);
+                   p_full = s_full + 8, pv_done = s_full + 24, q_full = s_full + 32, idle = s_full + 40;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * ST + 6);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dk = pool.dk, ps = 1 << pool.page_shift;
     const int steps = (k.end - k.begin + KT - 1) / KT;
@@ -729,7 +730,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 1); mbar_init(v_empty + 8 * i, 1); }
-        mbar_init(s_full, 1); mbar_init(p_full, 8); mbar_init(p_full + 8, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8);
+        mbar_init(s_full, 1); mbar_init(p_full, 8); mbar_init(p_full + 8, 8); mbar_init(pv_done, 1); mbar_init(q_full, 8); mbar_init(idle, 1);
         *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;         // the swizzled tiles need a 1024-byte aligned base
         if (*abort_flag) atomicCAS(&g_paged_attn_error, 0, 9 << 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -747,6 +748,10 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DP >> 3) << 17) | (uint32_t(128 >> 4) << 24);
     auto wait = [&](uint32_t bar, int parity, int code) -> bool { return mbar_wait(bar, parity & 1, abort_flag, code, &g_paged_attn_error); };
     auto wait_all = [&](uint32_t bar, int parity, int code) -> bool { return __all_sync(0xffffffffu, wait(bar, parity, code)); };
+    // what this block has under way is waited for before it ends, whoever gave up
+    auto drain = [&](uint32_t bar, int parity) {
+        if (!mbar_drain(bar, parity & 1)) { *abort_flag = 1; atomicCAS(&g_paged_attn_error, 0, 3 << 16); }
+    };
     // whether a page of the run is missing: looked over once, by every warp for itself
     bool gaps = false;
     for (int t = k.begin + lane * high; t < k.end; t += 32 * high) gaps |= pool.find(k.table, k.hk, t) < 0;
@@ -760,7 +765,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     if (warp == 0) {
         const int nowhere = pool.pages * pool.kv_heads * ps;    // a row behind the pool
         bool ok = !*abort_flag;
-        int row = box_of(0);
+        int row = box_of(0), k_loads = 0, v_loads = 0;          // steps whose loads have been issued
         for (int i = 0; ok && i < steps; ++i) {
             const int st = i % ST, use = i / ST, y = row < 0 ? nowhere : row;
             if (!(ok = wait_all(k_empty + 8 * st, use + 1, 1))) break;
@@ -770,6 +775,7 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
 #pragma unroll
                 for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sK) + st * Tc::TILE + j * Tc::SUB + lane * high * 128, tk, k_full + 8 * st, j * 64, y);
             }
+            k_loads = i + 1;
             row = box_of(i + 1);
             if (!(ok = wait_all(v_empty + 8 * st, use + 1, 2))) break;
             if (lane == 0) mbar_expect_tx(v_full + 8 * st, Tc::TILE);
@@ -778,11 +784,13 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
 #pragma unroll
                 for (int j = 0; j < NS; ++j) tma_load_2d(smem_u32(sV) + st * Tc::TILE + j * Tc::SUB + lane * high * 128, tv, v_full + 8 * st, j * 64, y);
             }
+            v_loads = i + 1;
         }
-        // nothing of this block's is under way when it ends: the last loads are waited for here, whoever gave up
-        if (lane == 0)
-            for (int i = max(0, steps - ST); i < steps; ++i)
-                if (!*abort_flag) { wait(k_full + 8 * (i % ST), i / ST, 3); wait(v_full + 8 * (i % ST), i / ST, 4); }
+        // a place's loads before its last ones have been used: only these can be under way
+        if (lane == 0) {
+            for (int i = max(0, k_loads - ST); i < k_loads; ++i) drain(k_full + 8 * (i % ST), i / ST);
+            for (int i = max(0, v_loads - ST); i < v_loads; ++i) drain(v_full + 8 * (i % ST), i / ST);
+        }
     } else if (warp == 1) {
         if (lane == 0) {
             bool ok = !*abort_flag && wait(q_full, 0, 5);
@@ -823,6 +831,8 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
                 if (!(ok = wait(pv_done, i, 15))) break;
                 if (!(ok = issue_s(i + 1))) break;
             }
+            umma_commit(idle);                                  // every product that was issued
+            drain(idle, 0);
         }
     } else {
         const int quad = warp & 3, half = (warp - 2) >> 2, row = quad * 32 + lane;
