@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
 // bandwidth a step of both blocks, of 4200 that it took, although the next step's S could then start half a P V earlier.  64 cached rows a step instead (an S of 128 x 64 takes the tensor core as long as one of 128 x 128) had the issue
 // of products as its bound: 2400 clocks for 64 rows and block, 12 products of 130 clocks.
 // Every wait is bounded; one that gives up raises a status word, the others see it, and the block drains: loads and products that
-// have been issued are waited for (again with a bound), and the two threads of a row leave together, at the barrier where they
-// compare notes.
+// have been issued are waited for (again with a bound), the two threads of a row leave together, at the barrier where they
+// compare notes, and the block's rows are NaN.
 __device__ int g_paged_attn_error = 0;
 
 template <int DP> struct AttnTc {
@@ -1017,6 +1017,10 @@ __device__ __forceinline__ void attend_tc(const PagedPool<bf16>& pool, const Pag
     }
     tc_fence_before();
     __syncthreads();
+    // a block that gave up has rows it did not write, or in part: NaN, which the join keeps, instead of an earlier call's
+    if (*abort_flag)
+        for (int idx = threadIdx.x; idx < k.rows * (dk / 4); idx += 320)
+            leave<bf16>(a, k, dk, a.by_vecs.div(idx), (idx - a.by_vecs.div(idx) * (dk / 4)) * 4, make_float4(NAN, NAN, NAN, NAN), -INFINITY, NAN);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Tc::TMEM_COLS) : "memory");

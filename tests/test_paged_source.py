@@ -45,3 +45,10 @@ def test_products_under_way_are_waited_for_before_their_tmem_is_freed():
 def test_a_drain_does_not_end_because_another_wait_gave_up():
     body = _function("tc_ptx.cuh", "bool mbar_drain(")
     assert "abort" not in body and "clock64() - t0 >" in body
+
+
+def test_rows_of_a_block_that_gave_up_are_nan():
+    """What such a block has not written, or only in part, must not reach the join as numbers of an earlier call."""
+    _, _, end = _roles()
+    written = re.search(r"if \(\*abort_flag\)\s*for \([^{}]*k\.rows[^{}]*leave<bf16>\(a, k, dk,[^{}]*make_float4\(NAN, NAN, NAN, NAN\), -INFINITY, NAN\);", end)
+    assert written and end.index("__syncthreads()") < written.start()
