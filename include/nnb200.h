@@ -488,7 +488,7 @@ int nnb200_paged_append(const nnb200_paged_kv* kv, int layer, const void* q, lon
  * seen, slope_h = 2^(-8 h / heads) as in nnb200_attention_forward.  q, out: rows of heads * head_dim values of the cache's type
  * with strides ldq, ldo; lse (NULL, or groups * group_size * heads): log of the sum of exponentials.  A query for which no row
  * has weight gives 0 and -inf.  Lengths beyond what the page tables hold count as what they hold; a stride of 0 is no prefix,
- * or no rows.  Accumulation and softmax in fp32; bf16: the weights are rounded to bf16 for their product with the values.
+ * or no rows.  Accumulation and softmax in fp32, divided by the sum of the weights at the end: values up to 2^80; bf16: the weights are rounded to bf16 for their product with the values.
  * scratch (16-byte aligned): nnb200_paged_attention_scratch_bytes, nothing in it needs to be set or kept; two calls that may
  * overlap need one each. */
 size_t nnb200_paged_attention_scratch_bytes(const nnb200_paged_kv* kv, int groups, int group_size, int heads, int prefix_stride,
@@ -504,7 +504,8 @@ int nnb200_paged_attention(const nnb200_paged_kv* kv, int layer, const void* q, 
  * token eos at its own score.  ended_out: the parent had ended, or the token is eos (-1: no such token).  -inf and NaN values
  * are no continuations, nor is anything of a row that holds NaN or +inf; places that nothing is left for get parent -1,
  * token -1, score -inf.  Up to 64 beams, beams * vocab below 2^31, vocab below 2^31 - 2^16.  Values are compared in 64 bits;
- * the normaliser is summed in 64 bits from exponentials in 32, off by less than 2.3e-6, and exact where that decides the order. */
+ * the normaliser is summed in 64 bits from exponentials in 32, off by less than 2.3e-6, and exact where that decides the order.
+ * Where 64 bits do not tell continuations of a beam apart although their logits differ (a score of -3e38, say), any of them may come. */
 size_t nnb200_beam_select_scratch_bytes(int groups, int beams, int vocab, int n);
 int nnb200_beam_select(const void* logits, long long ld, int dtype, int groups, int beams, int vocab, const float* scores,
                        const int32_t* ended, int eos, int n, int32_t* parent, int32_t* token, float* scores_out, int32_t* ended_out,

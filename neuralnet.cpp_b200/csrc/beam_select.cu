@@ -16,9 +16,10 @@
 // bound are looked at again.  (Comparing each logit with a running threshold on the way took 2000 of a tile's 3800 clocks: with
 // 1000 logits a warp and tile somebody always has one.)  The second kernel, already resident when the first ends, joins the spans'
 // sums and picks from the rows' lists.
-// 64 groups of 8 beams over 32768 bf16 logits, 16 continuations: 21.4 us, of which the picking is 6 and the reading about 12 (a tile of
-// 4096 takes a block 1400 clocks beside three others; its exponentials alone, at 16 an SM and clock, take 1024 of them).  One group
-// of 4 beams over 4096: 7.0 us, two launches of a few dependent steps.
+// 64 groups of 8 beams over 32768 bf16 logits, 16 continuations: 21.3 us.  Its 512 blocks are one wave: 11.7 us until the last has been
+// through its eight tiles (the exponentials alone, at 16 an SM and clock and with four blocks an SM, take 4.3, the copy rate 5.2),
+// 3.7 for what ends a span (the bound 1.3, the shares that reach it 1.3, sorting the list 0.7, the sum 0.4), 0.8 to the second kernel
+// and 5 to 6 in it.  One group of 4 beams over 4096: 7.1 us, two launches of a few dependent steps.
 #include <algorithm>
 
 #include "common.cuh"

@@ -329,7 +329,7 @@ __device__ __forceinline__ void attend_bf16(const PagedPool<bf16>& pool, const P
             for (int j = 0; j < 4; ++j) { s[n][j] = exp2_fast(fmaf(s[n][j], mul, -ref[j >> 1])); l[j >> 1] += s[n][j]; }
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
-            // the weights are rounded to bf16 for the tensor cores (their sum is not): 2^-9 of a weight, what rounding V costs too
+            // the weights are rounded to bf16 for the tensor cores (their sum is not): 2^-8 of a weight at most, what rounding V costs too
             const uint32_t p[4] = {pack_bf16x2(s[n][0], s[n][1]), pack_bf16x2(s[n][2], s[n][3]), pack_bf16x2(s[n + 1][0], s[n + 1][1]), pack_bf16x2(s[n + 1][2], s[n + 1][3])};
 #pragma unroll
             for (int d = 0; d < ND; d += 2) {
@@ -576,7 +576,7 @@ __device__ __forceinline__ void stream_bf16(const PagedPool<bf16>& pool, const P
                 float e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) { e[j] = exp2_fast(fmaf(s[x][n][j], mul, -ref[n][j & 1])); l[n][j & 1] += e[j]; }
-                // the weights are rounded to bf16 for the tensor cores (their sum is not): half a step of 2^-8, what rounding V costs too
+                // the weights are rounded to bf16 for the tensor cores (their sum is not): 2^-8 of a weight at most, what rounding V costs too
                 p[n][0] = transposed8x8(pack_bf16x2(e[0], e[1]));
                 p[n][1] = transposed8x8(pack_bf16x2(e[2], e[3]));
             }
@@ -669,8 +669,9 @@ __global__ void __launch_bounds__(128) paged_attn_bf16_kernel(PagedPool<bf16> po
 }
 
 // ---------------------------------------------------------------- bf16: tcgen05 tiles
-// More than 16 query rows on the 5th-generation tensor cores: 128 rows (those that are not there are zero) against 128 cached
-// rows a step.  S = Q K' (128 x 128) goes to TMEM, O (128 x DP) stays in TMEM across steps.
+// More than 64 query rows of heads up to 64 wide, more than 16 of heads up to 128, on the 5th-generation tensor cores: 128 rows (those
+// that are not there are zero) against 128 cached rows a step.  S = Q K' (128 x 128) goes to TMEM, O (128 x DP) stays in TMEM across
+// steps.
 //   warp 0     looks up the step's pages and loads their rows by TMA, a box of a page (64 rows of a larger one) per lane; pages
 //              that are not there are loaded from behind the pool's end, where TMA fills in zeros
 //   warp 1     issues the products: S, and O += P V in two halves of 64 cached rows
